@@ -278,6 +278,12 @@ class Runtime:
         _check(_calls.sample_rows_into(self.h, logits, rows, vocab, temperature, 0 if top_k is None else top_k, top_p, seed, counter, seeds,
                                        counters, tokens))
 
+    def logprobs_into(self, logits, rows, vocab, targets=None, logprobs=None, entropy=None, top=0, top_tokens=None, top_logprobs=None, row_stride=None):
+        """Log probability of each row's target token, entropy and the `top` (0 to 32) most likely tokens of each row of logits with
+        their log probabilities, into device tensors (f32; tokens and targets 32-bit). Rows are row_stride values apart."""
+        _check(_calls.logprobs_into(self.h, logits, rows, vocab, vocab if row_stride is None else row_stride, targets, logprobs, entropy, top, top_tokens,
+                                    top_logprobs))
+
     def kv_attention_into(self, pool, layer, seqs, batch, active, advance, q, k, v, q_heads, tokens, scale, op_window=None,
                           pool_window=None, out=None):
         arr = (C.c_void_p * max(len(seqs), 1))(*[s.h for s in seqs])

@@ -143,6 +143,19 @@ PyObject* sample_rows_into(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return finish(a, [&] { return etc_sample_rows_into(rt, logits, rows, vocab, temperature, top_k, top_p, seed, counter, seeds, counters, tokens); });
 }
 
+PyObject* logprobs_into(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Arguments a(args, n, 11);
+  auto* rt = a.pointer<etc_runtime>();
+  const float* logits = a.pointer<float>();
+  const int64_t rows = a.wide(), vocab = a.wide(), stride = a.wide();
+  const uint32_t* targets = a.pointer<uint32_t>();
+  float *logprobs = a.pointer<float>(), *entropy = a.pointer<float>();
+  const int top = a.narrow();
+  uint32_t* top_tokens = a.pointer<uint32_t>();
+  float* top_logprobs = a.pointer<float>();
+  return finish(a, [&] { return etc_logprobs_into(rt, logits, rows, vocab, stride, targets, logprobs, entropy, top, top_tokens, top_logprobs); });
+}
+
 PyObject* paged_attention_into(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Arguments a(args, n, 14);
   auto* rt = a.pointer<etc_runtime>();
@@ -163,7 +176,7 @@ PyObject* paged_attention_into(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define CALL(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {CALL(dequantize_into), CALL(quantize_into),    CALL(qlinear_into), CALL(qlinear_tiled_into),
-                           CALL(sample_rows_into), CALL(paged_attention_into), {nullptr, nullptr, 0, nullptr}};
+                           CALL(sample_rows_into), CALL(logprobs_into), CALL(paged_attention_into), {nullptr, nullptr, 0, nullptr}};
 #undef CALL
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", "Operators of the C ABI without ctypes.", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -42,7 +42,9 @@ struct DeviceStatus {
   long long bound;             // rows / vocabulary
   long long reserved;
 };
-enum : unsigned long long { kStatusNone = 0, kStatusIndexOutOfRange = 1, kStatusNonFiniteLogit = 2 };
+enum : unsigned long long {
+  kStatusNone = 0, kStatusIndexOutOfRange = 1, kStatusNonFiniteLogit = 2, kStatusTargetOutOfRange = 5, kStatusBadLogprobLogit = 6
+};
 
 constexpr uint32_t kRuntimeMagic = 0x45544352;  // "ETCR"
 constexpr uint32_t kPoolMagic = 0x45544350;

@@ -202,6 +202,12 @@ cudaError_t launch_argmax(const float* logits, int64_t rows, int64_t vocab, uint
 cudaError_t launch_sample_rows(const float* logits, int64_t rows, int64_t vocab, double temperature, int64_t top_k, double top_p,
                                uint64_t seed, uint64_t counter, const uint64_t* seeds, const uint64_t* counters, uint32_t* tokens,
                                DeviceStatus* status, cudaStream_t stream);
+// Per row of logits: log probability of its target, entropy, the `top` most likely tokens (logprobs.cu). targets with logprobs, and
+// entropy, may be null; top may be 0.
+constexpr int kMaxAlternatives = 32;
+cudaError_t launch_logprobs(const float* logits, int64_t rows, int64_t vocab, int64_t row_stride, const uint32_t* targets, float* logprobs,
+                            float* entropy, int top, uint32_t* top_tokens, float* top_logprobs, DeviceStatus* status, int sm_count,
+                            cudaStream_t stream);
 cudaError_t launch_embedding_f32(const void* indexes, int index_is_i64, int64_t count, const float* table, int64_t rows,
                                  int64_t columns, float* out, DeviceStatus* status, cudaStream_t stream);
 // Copy row (advance-1) of each lane's [T, width] block into [lanes, width] (LastTokenRow).

@@ -41,6 +41,14 @@ etc_status validate_sampling(int64_t length, double temperature, int64_t top_k, 
   return ETC_OK;
 }
 
+etc_status validate_logprobs(int64_t vocab, int top) {
+  if (vocab <= 0) return fail(ETC_EXECUTION, "logprobs: logits must be non-empty");
+  if (vocab > 1048576) return fail(ETC_EXECUTION, "logprobs: vocabulary " + std::to_string(vocab) + " exceeds limit 1048576");
+  const int64_t most = std::min<int64_t>(kMaxAlternatives, vocab);
+  if (top < 0 || top > most) return fail(ETC_EXECUTION, "logprobs: the number of alternatives must be in [0, " + std::to_string(most) + "], got " + std::to_string(top));
+  return ETC_OK;
+}
+
 etc_status make_inv_freq(etc_runtime* rt, double theta, int head_dim, double** out_device) {
   // theta^(-2j/D) with the host pow(), as rotary_forward_into_impl evaluates it (composed.rs:2712-2716)
   const int half = head_dim / 2;
@@ -432,6 +440,23 @@ etc_status etc_sample_row(etc_runtime* rt, const float* d_logits, int64_t vocab,
   if (e != cudaSuccess) return fail(ETC_TRANSFER, std::string("readback failed: ") + cudaGetErrorString(e));
   ETC_TRY(rt->check_status());  // synchronises; a non-finite logit surfaces here
   *out_token = *rt->h_sampled;
+  return ETC_OK;
+}
+
+etc_status etc_logprobs_into(etc_runtime* rt, const float* d_logits, int64_t rows, int64_t vocab, int64_t row_stride, const uint32_t* d_targets,
+                             float* d_logprobs, float* d_entropy, int top, uint32_t* d_top_tokens, float* d_top_logprobs) {
+  ETC_TRY(activate(rt));
+  ETC_TRY(validate_logprobs(vocab, top));
+  if (rows < 0 || rows > (1 << 27)) return fail(ETC_INVALID_ARGUMENT, "logprobs: the number of rows must be in 0.." + std::to_string(1 << 27));
+  if (row_stride < vocab) return fail(ETC_INVALID_ARGUMENT, "logprobs: a row stride of " + std::to_string(row_stride) + " is shorter than a row");
+  if (rows > 0 && row_stride > INT64_MAX / 4 / rows) return fail(ETC_INVALID_ARGUMENT, "logprobs: logits byte size overflow");
+  if (rows == 0) return ETC_OK;
+  if (!d_logits || (d_targets == nullptr) != (d_logprobs == nullptr) || (top > 0 && (!d_top_tokens || !d_top_logprobs)))
+    return fail(ETC_INVALID_ARGUMENT, "logprobs: logits, targets with log probabilities and buffers for the alternatives must be device buffers");
+  if (!d_logprobs && !d_entropy && top == 0) return ETC_OK;
+  ETC_CUDA(launch_logprobs(d_logits, rows, vocab, row_stride, d_targets, d_logprobs, d_entropy, top, d_top_tokens, d_top_logprobs, rt->d_status,
+                           rt->sm_count, rt->stream));
+  rt->launches++;
   return ETC_OK;
 }
 

@@ -251,6 +251,20 @@ ETC_API etc_status etc_sample_rows_into(etc_runtime* rt, const float* d_logits, 
 ETC_API etc_status etc_sample_row(etc_runtime* rt, const float* d_logits, int64_t vocab, double temperature,
                                   int64_t top_k, double top_p, uint64_t seed, uint64_t counter, uint32_t* out_token);
 
+/* Scores of logits rows (no counterpart in the reference, whose programs read logits back and do this on the host). For each of the
+ * `rows` rows of `vocab` f32 logits, row_stride apart (in values, >= vocab; rows may start on any 4-byte boundary):
+ *   d_logprobs[r] = log softmax(row)[d_targets[r]]      (both given or both NULL)
+ *   d_entropy[r]  = -sum p ln p, in nats                (may be NULL)
+ *   d_top_tokens / d_top_logprobs [rows, top]: the most likely tokens, largest first, of equal logits the lower token first, and
+ *                   their log probabilities             (top in 0..min(32, vocab); NULL with 0)
+ * -inf logits (barred tokens) have log probability -inf; a row of nothing else has NaN log probabilities and entropy and its first
+ * tokens as alternatives. Sums are f32 within some 250 values and f64 above. Asynchronous, capturable, nothing allocated. A
+ * target >= vocab (its log probability is NaN) is reported at the next synchronising call as ETC_EXECUTION "logprobs: target {t}
+ * is outside 0..{vocab}", a NaN or +inf logit as "logprobs: logit {i} of row {r} is NaN or +inf" (that row's results mean nothing). */
+ETC_API etc_status etc_logprobs_into(etc_runtime* rt, const float* d_logits, int64_t rows, int64_t vocab, int64_t row_stride,
+                                     const uint32_t* d_targets, float* d_logprobs, float* d_entropy, int top,
+                                     uint32_t* d_top_tokens, float* d_top_logprobs);
+
 /* ------------------------------------------------------------------------------------------
  * Paged KV pool and sequences (NativeKvPool / NativeKvSequence,
  * crates/runtime-cpu/src/napi/mod.rs:3632-3947; native-addon.ts:193-220).

@@ -298,6 +298,19 @@ extern "C" {
         counter: u64,
         out_token: *mut u32,
     ) -> EtcStatus;
+    pub fn etc_logprobs_into(
+        rt: *mut EtcRuntime,
+        d_logits: *const f32,
+        rows: i64,
+        vocab: i64,
+        row_stride: i64,
+        d_targets: *const u32,
+        d_logprobs: *mut f32,
+        d_entropy: *mut f32,
+        top: c_int,
+        d_top_tokens: *mut u32,
+        d_top_logprobs: *mut f32,
+    ) -> EtcStatus;
     pub fn etc_pool_create(
         rt: *mut EtcRuntime,
         layers: c_int,
