@@ -20,7 +20,7 @@ import weakref
 import numpy as np
 
 from . import _lib
-from ._lib import DecoderConfig
+from ._lib import DecoderConfig, RopeConfig
 
 # status classes (include/et_cuda.h) -> BackendError.reason (packages/core/src/Runtime.ts:129-143)
 REASONS = {
@@ -31,6 +31,7 @@ Q4_0, Q8_0, Q2_K, Q3_K, Q4_K, Q5_K, Q6_K, F32_CODEC = 2, 8, 10, 11, 12, 13, 14, 
 KV_F32, KV_F16, KV_BF16, KV_U8 = 0, 1, 2, 3
 HALF_SPLIT, INTERLEAVED_PAIRS = 0, 1
 EPILOGUE_NONE, EPILOGUE_RESIDUAL, EPILOGUE_SWIGLU = 0, 1, 2
+ROPE_SCALINGS = {"none": 0, "linear": 1, "llama3": 2, "yarn": 3}
 NO_WINDOW = -1
 (W_TOK_EMBD, W_ATTN_NORM, W_Q, W_K, W_V, W_O, W_FFN_NORM, W_GATE, W_UP, W_DOWN, W_OUT_NORM, W_HEAD) = range(12)
 
@@ -257,6 +258,13 @@ class Runtime:
     def rope_into(self, x, offsets, n_offsets, theta, layout, batch, heads, steps, head_dim, out):
         _check(self.L.etc_rope_into(self.h, _ptr(x), _ptr(offsets), n_offsets, theta, layout, batch, heads, steps, head_dim, _ptr(out)))
 
+    def rotary_into(self, table, x, offsets, batch, heads, steps, out, x_strides=None, out_strides=None, n_offsets=None):
+        """Rotates x [batch, heads, steps, head_dim] by a RotaryTable into out; strides of (batch, heads, steps) in values, dense
+        where they are not given. Step s of batch entry b is at position offsets[b] + s (device i64, one for all with n_offsets=1)."""
+        dense = (heads * steps * table.head_dim, steps * table.head_dim, table.head_dim)
+        _check(_calls.rotary_into(self.h, table.h, x, *(dense if x_strides is None else x_strides), offsets, batch if n_offsets is None else n_offsets, batch,
+                                  heads, steps, out, *(dense if out_strides is None else out_strides)))
+
     def swiglu_into(self, gate, up, n, out):
         _check(self.L.etc_swiglu_into(self.h, _ptr(gate), _ptr(up), n, _ptr(out)))
 
@@ -321,6 +329,54 @@ class Runtime:
 def peer_region_bytes(capacity: int, world: int) -> int:
     """Bytes of one rank's exchange region for peer all-reduces of up to `capacity` floats among `world` ranks."""
     return int(_lib.load().etc_peer_region_bytes(capacity, world))
+
+
+def rope_config(head_dim, *, rotary_dim=None, theta=10000.0, layout=HALF_SPLIT, scaling="none", factor=1.0, original_context=0, low_freq_factor=1.0,
+                high_freq_factor=4.0, beta_fast=32.0, beta_slow=1.0, attention_factor=0.0) -> RopeConfig:
+    """How positions are rotated: the first rotary_dim values of a head (all by default), at frequencies scaled by the rule `scaling`
+    ("none", "linear", "llama3", "yarn") for contexts `factor` times the trained one. attention_factor 0: by the rule."""
+    if scaling not in ROPE_SCALINGS:
+        raise BackendError(4, f"rotary: unknown scaling {scaling!r}")
+    return RopeConfig(head_dim, head_dim if rotary_dim is None else rotary_dim, layout, ROPE_SCALINGS[scaling], theta, factor, original_context,
+                      low_freq_factor, high_freq_factor, beta_fast, beta_slow, attention_factor)
+
+
+def _divisors(config, divisors):
+    if divisors is None:
+        return None
+    d = np.ascontiguousarray(divisors, dtype=np.float32).reshape(-1)
+    if d.size != config.rotary_dim // 2:
+        raise BackendError(4, f"rotary: {d.size} frequency divisors for {config.rotary_dim // 2} pairs")
+    return d
+
+
+def rope_frequencies(config: RopeConfig, divisors=None):
+    """(angle per position of each pair, f64; factor on what is rotated): host arithmetic, no device."""
+    d = _divisors(config, divisors)
+    f, magnitude = np.zeros(max(config.rotary_dim // 2, 1)), C.c_double(0.0)
+    _check(_lib.load().etc_rope_frequencies(C.byref(config), _ptr(d), _ptr(f), C.byref(magnitude)))
+    return f, magnitude.value
+
+
+class RotaryTable:
+    """Frequencies of rotary positions on the device, for Runtime.rotary_into. Keywords as rope_config's; divisors: one per pair."""
+
+    def __init__(self, rt: Runtime, head_dim, divisors=None, **rule):
+        self.rt, self.config, self.head_dim = rt, rope_config(head_dim, **rule), head_dim
+        d, h = _divisors(self.config, divisors), C.c_void_p()
+        _check(rt.L.etc_rotary_create(rt.h, C.byref(self.config), _ptr(d), C.byref(h)))
+        self.h = h.value
+
+    def close(self):
+        if getattr(self, "h", None) and getattr(self.rt, "h", None):
+            self.rt.L.etc_rotary_destroy(self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class QWeight:

@@ -29,6 +29,11 @@ class DecoderConfig(C.Structure):
     ]
 
 
+class RopeConfig(C.Structure):
+    _fields_ = [("head_dim", I), ("rotary_dim", I), ("layout", I), ("scaling", I), ("theta", D), ("factor", D), ("original_context", D),
+                ("low_freq_factor", D), ("high_freq_factor", D), ("beta_fast", D), ("beta_slow", D), ("attention_factor", D)]
+
+
 class Capabilities(C.Structure):
     _fields_ = [("dtype_mask", U32), ("feature_mask", U32), ("device_ordinal", I), ("sm_count", I), ("compute_major", I),
                 ("compute_minor", I), ("device_memory_bytes", U64), ("device_name", C.c_char * 128)]
@@ -66,6 +71,10 @@ SIGNATURES = {
     "etc_linear_f32_into": (None, [P, P, I64, I64, P, I64, P, P]),
     "etc_rmsnorm_into": (None, [P, P, P, D, I64, I64, P]),
     "etc_rope_into": (None, [P, P, P, I64, D, I, I64, I64, I64, I64, P]),
+    "etc_rope_frequencies": (None, [P, P, P, P]),
+    "etc_rotary_create": (None, [P, P, P, P]),
+    "etc_rotary_destroy": (None, [P]),
+    "etc_rotary_into": (None, [P, P, P, I64, I64, I64, P, I64, I64, I64, I64, P, I64, I64, I64]),
     "etc_swiglu_into": (None, [P, P, P, I64, P]),
     "etc_add_into": (None, [P, P, P, I64, P]),
     "etc_argmax_into": (None, [P, P, I64, I64, P]),

@@ -143,6 +143,19 @@ PyObject* sample_rows_into(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return finish(a, [&] { return etc_sample_rows_into(rt, logits, rows, vocab, temperature, top_k, top_p, seed, counter, seeds, counters, tokens); });
 }
 
+PyObject* rotary_into(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Arguments a(args, n, 15);
+  auto* rt = a.pointer<etc_runtime>();
+  const auto* rotary = a.pointer<etc_rotary>();
+  const float* x = a.pointer<float>();
+  const int64_t xb = a.wide(), xh = a.wide(), xs = a.wide();
+  const int64_t* offsets = a.pointer<int64_t>();
+  const int64_t n_offsets = a.wide(), batch = a.wide(), heads = a.wide(), steps = a.wide();
+  float* out = a.pointer<float>();
+  const int64_t ob = a.wide(), oh = a.wide(), os = a.wide();
+  return finish(a, [&] { return etc_rotary_into(rt, rotary, x, xb, xh, xs, offsets, n_offsets, batch, heads, steps, out, ob, oh, os); });
+}
+
 PyObject* logprobs_into(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Arguments a(args, n, 11);
   auto* rt = a.pointer<etc_runtime>();
@@ -176,7 +189,7 @@ PyObject* paged_attention_into(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define CALL(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {CALL(dequantize_into), CALL(quantize_into),    CALL(qlinear_into), CALL(qlinear_tiled_into),
-                           CALL(sample_rows_into), CALL(logprobs_into), CALL(paged_attention_into), {nullptr, nullptr, 0, nullptr}};
+                           CALL(sample_rows_into), CALL(rotary_into), CALL(logprobs_into), CALL(paged_attention_into), {nullptr, nullptr, 0, nullptr}};
 #undef CALL
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", "Operators of the C ABI without ctypes.", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -51,6 +51,7 @@ constexpr uint32_t kPoolMagic = 0x45544350;
 constexpr uint32_t kSeqMagic = 0x45544353;
 constexpr uint32_t kWeightMagic = 0x45544357;
 constexpr uint32_t kDecoderMagic = 0x45544344;
+constexpr uint32_t kRotaryMagic = 0x4554434f;
 
 }  // namespace etc
 

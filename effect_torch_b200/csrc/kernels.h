@@ -192,6 +192,18 @@ cudaError_t launch_rmsnorm(const float* x, const float* weight, double eps, int6
                            cudaStream_t stream);
 cudaError_t launch_rope(const float* x, const int64_t* offsets, int64_t n_offsets, const double* inv_freq, int layout,
                         int64_t batch, int64_t heads, int64_t steps, int64_t head_dim, float* out, cudaStream_t stream);
+// Rotary positions from a table of frequencies (rotary.cu). Strides of [batch, heads, steps], in values; head values are contiguous.
+struct RotaryArgs {
+  const float* x;
+  float* out;
+  int64_t x_stride[3], out_stride[3];
+  const int64_t* offsets;
+  int64_t n_offsets;
+  int heads, steps, head_dim, rotary_half, layout, in_place;
+  const double* half_turns;  // [rotary_half] angle per position / pi
+  float magnitude;
+};
+cudaError_t launch_rotary(const RotaryArgs& args, int64_t batch, int sm_count, cudaStream_t stream);
 cudaError_t launch_swiglu(const float* gate, const float* up, int64_t n, float* out, int exact, cudaStream_t stream);
 cudaError_t launch_add(const float* a, const float* b, int64_t n, float* out, cudaStream_t stream);
 cudaError_t launch_argmax(const float* logits, int64_t rows, int64_t vocab, uint32_t* tokens, DeviceStatus* status,

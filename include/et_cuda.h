@@ -75,6 +75,24 @@ typedef enum etc_kv_dtype { ETC_KV_F32 = 0, ETC_KV_F16 = 1, ETC_KV_BF16 = 2, ETC
 /* RotaryLayout (crates/runtime-cpu/src/composed.rs:2714-2717). */
 typedef enum etc_rope_layout { ETC_ROPE_HALF_SPLIT = 0, ETC_ROPE_INTERLEAVED_PAIRS = 1 } etc_rope_layout;
 
+/* How the frequencies of rotary positions are scaled beyond the trained context. */
+typedef enum etc_rope_scaling {
+  ETC_ROPE_SCALING_NONE = 0,
+  ETC_ROPE_SCALING_LINEAR = 1, /* all frequencies / factor */
+  ETC_ROPE_SCALING_LLAMA3 = 2, /* pairs below low_freq_factor turns in original_context / factor, above high_freq_factor as trained, between: blended */
+  ETC_ROPE_SCALING_YARN = 3    /* pairs ramp from as trained (beta_fast turns) to / factor (beta_slow turns); attention factor 0.1 ln factor + 1 */
+} etc_rope_scaling;
+typedef struct etc_rope_config {
+  int head_dim, rotary_dim;     /* the first rotary_dim values of a head are rotated (even), the others pass */
+  int layout;                   /* etc_rope_layout, over the rotated values */
+  int scaling;                  /* etc_rope_scaling */
+  double theta, factor;         /* factor >= 1; unused without scaling */
+  double original_context;      /* llama3, yarn: the trained context */
+  double low_freq_factor, high_freq_factor; /* llama3 */
+  double beta_fast, beta_slow;  /* yarn */
+  double attention_factor;      /* multiplies what is rotated; 0: by the scaling's rule (1 without one) */
+} etc_rope_config;
+
 typedef enum etc_index_dtype { ETC_INDEX_U32 = 0, ETC_INDEX_I64 = 1 } etc_index_dtype;
 
 typedef struct etc_runtime etc_runtime;
@@ -82,6 +100,7 @@ typedef struct etc_pool etc_pool;
 typedef struct etc_seq etc_seq;
 typedef struct etc_qweight etc_qweight;
 typedef struct etc_decoder etc_decoder;
+typedef struct etc_rotary etc_rotary;
 
 #define ETC_NO_WINDOW (-1)
 
@@ -228,6 +247,22 @@ ETC_API etc_status etc_rmsnorm_into(etc_runtime* rt, const float* d_x, const flo
 ETC_API etc_status etc_rope_into(etc_runtime* rt, const float* d_x, const int64_t* d_offsets, int64_t n_offsets,
                                  double theta, etc_rope_layout layout, int64_t batch, int64_t heads, int64_t steps,
                                  int64_t head_dim, float* d_out);
+/* Rotary positions with scaled frequencies, of part of a head or all of it, in either layout (the reference rotates whole heads at the
+ * plain frequencies). etc_rope_frequencies is the rule alone, host arithmetic: the angle per position of each of the rotary_dim / 2
+ * pairs, theta^(-2j / rotary_dim) / h_divisors[j] (may be NULL; what GGUF files keep as rope_freqs) and then scaled, and the factor on
+ * what is rotated. Bad configurations are ETC_COMPILATION "rotary: ...". A table keeps them on the device. */
+ETC_API etc_status etc_rope_frequencies(const etc_rope_config* config, const float* h_divisors, double* h_inv_freq,
+                                        double* out_attention_factor);
+ETC_API etc_status etc_rotary_create(etc_runtime* rt, const etc_rope_config* config, const float* h_divisors, etc_rotary** out);
+ETC_API etc_status etc_rotary_destroy(etc_rotary* rotary);
+/* Rotates f32 [batch, heads, steps, head_dim], whose first three axes may lie in memory in any order: strides in values, those of out at
+ * least a head where the axis is longer than one (the stride of an axis of one is ignored), x may repeat (stride 0). Step s of
+ * batch entry b is at position d_offsets[b] + s (n_offsets 1: d_offsets[0] + s). In place (d_out == d_x) needs equal
+ * strides; buffers must not overlap otherwise. Angles are exact to f64 at any position, sines and cosines f32. Asynchronous, capturable. */
+ETC_API etc_status etc_rotary_into(etc_runtime* rt, const etc_rotary* rotary, const float* d_x, int64_t x_batch_stride,
+                                   int64_t x_head_stride, int64_t x_step_stride, const int64_t* d_offsets, int64_t n_offsets,
+                                   int64_t batch, int64_t heads, int64_t steps, float* d_out, int64_t out_batch_stride,
+                                   int64_t out_head_stride, int64_t out_step_stride);
 /* silu(gate) * up with sigmoid(x) = tanh(x/2)/2 + 1/2 (packages/core/src/Tensor.ts:1240-1245, 1537-1540). */
 ETC_API etc_status etc_swiglu_into(etc_runtime* rt, const float* d_gate, const float* d_up, int64_t n, float* d_out);
 ETC_API etc_status etc_add_into(etc_runtime* rt, const float* d_a, const float* d_b, int64_t n, float* d_out);

@@ -67,7 +67,7 @@ pub const ETC_NO_WINDOW: i64 = -1;
 macro_rules! opaque {
     ($($name:ident),*) => { $( #[repr(C)] pub struct $name { _private: [u8; 0] } )* };
 }
-opaque!(EtcRuntime, EtcPool, EtcSeq, EtcQweight, EtcDecoder, EtcGguf);
+opaque!(EtcRuntime, EtcPool, EtcSeq, EtcQweight, EtcDecoder, EtcGguf, EtcRotary);
 
 /// `etc_capabilities`.
 #[repr(C)]
@@ -113,6 +113,30 @@ pub struct EtcLane {
     pub advance: c_int,
     pub start: c_int,
     pub table_offset: c_int,
+}
+
+/// `etc_rope_scaling`.
+pub const ETC_ROPE_SCALING_NONE: c_int = 0;
+pub const ETC_ROPE_SCALING_LINEAR: c_int = 1;
+pub const ETC_ROPE_SCALING_LLAMA3: c_int = 2;
+pub const ETC_ROPE_SCALING_YARN: c_int = 3;
+
+/// `etc_rope_config`: the rotated part of a head, its layout and how its frequencies are scaled.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct EtcRopeConfig {
+    pub head_dim: c_int,
+    pub rotary_dim: c_int,
+    pub layout: c_int,
+    pub scaling: c_int,
+    pub theta: f64,
+    pub factor: f64,
+    pub original_context: f64,
+    pub low_freq_factor: f64,
+    pub high_freq_factor: f64,
+    pub beta_fast: f64,
+    pub beta_slow: f64,
+    pub attention_factor: f64,
 }
 
 #[link(name = "etcuda")]
@@ -257,6 +281,31 @@ extern "C" {
         steps: i64,
         head_dim: i64,
         d_out: *mut f32,
+    ) -> EtcStatus;
+    pub fn etc_rope_frequencies(
+        config: *const EtcRopeConfig,
+        h_divisors: *const f32,
+        h_inv_freq: *mut f64,
+        out_attention_factor: *mut f64,
+    ) -> EtcStatus;
+    pub fn etc_rotary_create(rt: *mut EtcRuntime, config: *const EtcRopeConfig, h_divisors: *const f32, out: *mut *mut EtcRotary) -> EtcStatus;
+    pub fn etc_rotary_destroy(rotary: *mut EtcRotary) -> EtcStatus;
+    pub fn etc_rotary_into(
+        rt: *mut EtcRuntime,
+        rotary: *const EtcRotary,
+        d_x: *const f32,
+        x_batch_stride: i64,
+        x_head_stride: i64,
+        x_step_stride: i64,
+        d_offsets: *const i64,
+        n_offsets: i64,
+        batch: i64,
+        heads: i64,
+        steps: i64,
+        d_out: *mut f32,
+        out_batch_stride: i64,
+        out_head_stride: i64,
+        out_step_stride: i64,
     ) -> EtcStatus;
     pub fn etc_swiglu_into(
         rt: *mut EtcRuntime,
