@@ -28,7 +28,7 @@ REASONS = {
     5: "execution-failed", 6: "transfer-failed", 7: "cancelled", 8: "closed-runtime", 9: "invalid-argument",
 }
 Q4_0, Q8_0, Q2_K, Q3_K, Q4_K, Q5_K, Q6_K, F32_CODEC = 2, 8, 10, 11, 12, 13, 14, 0
-KV_F32, KV_F16, KV_BF16, KV_U8 = 0, 1, 2, 3
+KV_F32, KV_F16, KV_BF16, KV_U8, KV_Q4 = 0, 1, 2, 3, 4
 HALF_SPLIT, INTERLEAVED_PAIRS = 0, 1
 EPILOGUE_NONE, EPILOGUE_RESIDUAL, EPILOGUE_SWIGLU = 0, 1, 2
 ROPE_SCALINGS = {"none": 0, "linear": 1, "llama3": 2, "yarn": 3}
@@ -325,6 +325,15 @@ class Runtime:
         _check(_calls.paged_attention_into(self.h, pool.h, layer, lanes, tables, batch, max_pages, q, q_heads, scale,
                                            NO_WINDOW if op_window is None else op_window, out, scratch, scratch_bytes))
 
+    def paged_append_into(self, pool, layer, lanes, tables, batch, tokens, k, v):
+        """New K / V rows [batch, kv_heads, tokens, head_dim] into the pages of device-resident lanes [batch, 4] i32 = (cursor, advance, start,
+        table offset) and block tables (asynchronous, capturable); positions cursor .. cursor + advance - 1."""
+        _check(_calls.paged_append_into(self.h, pool.h, layer, lanes, tables, batch, tokens, k, v))
+
+    def pool_rows_into(self, pool, layer, which, rows, n, out):
+        """The values of n cached rows (device u32 row numbers) of a layer's K (which 0) or V (1), f32 [n, kv_heads * head_dim]."""
+        _check(_calls.pool_rows_into(self.h, pool.h, layer, which, rows, n, out))
+
 
 def peer_region_bytes(capacity: int, world: int) -> int:
     """Bytes of one rank's exchange region for peer all-reduces of up to `capacity` floats among `world` ranks."""
@@ -470,6 +479,12 @@ class NativeKvPool:
 
     def makeSequence(self) -> "NativeKvSequence":
         return NativeKvSequence(self)
+
+    def attention_scratch_bytes(self, batch: int, q_heads: int, max_pages: int) -> int:
+        """Scratch that Runtime.paged_attention_into needs on this pool for lanes that attend over at most max_pages pages."""
+        n = C.c_size_t(0)
+        _check(self.rt.L.etc_paged_attention_scratch_bytes(self.h, batch, q_heads, max_pages, C.byref(n)))
+        return n.value
 
     def read_rows(self, layer: int, which: int, rows) -> np.ndarray:
         rows = np.ascontiguousarray(rows, dtype=np.uint32)

@@ -187,9 +187,32 @@ PyObject* paged_attention_into(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return finish(a, [&] { return etc_paged_attention_into(rt, pool, layer, lanes, tables, batch, max_pages, q, q_heads, scale, window, out, scratch, scratch_bytes); });
 }
 
+PyObject* paged_append_into(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Arguments a(args, n, 9);
+  auto* rt = a.pointer<etc_runtime>();
+  auto* pool = a.pointer<etc_pool>();
+  const int layer = a.narrow();
+  const auto* lanes = a.pointer<etc_lane>();
+  const int* tables = a.pointer<int>();
+  const int batch = a.narrow(), tokens = a.narrow();
+  const float *k = a.pointer<float>(), *v = a.pointer<float>();
+  return finish(a, [&] { return etc_paged_append_into(rt, pool, layer, lanes, tables, batch, tokens, k, v); });
+}
+
+PyObject* pool_rows_into(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  Arguments a(args, n, 7);
+  auto* rt = a.pointer<etc_runtime>();
+  auto* pool = a.pointer<etc_pool>();
+  const int layer = a.narrow(), which = a.narrow();
+  const uint32_t* rows = a.pointer<uint32_t>();
+  const int64_t count = a.wide();
+  float* out = a.pointer<float>();
+  return finish(a, [&] { return etc_pool_rows_into(rt, pool, layer, which, rows, count, out); });
+}
+
 #define CALL(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {CALL(dequantize_into), CALL(quantize_into),    CALL(qlinear_into), CALL(qlinear_tiled_into),
-                           CALL(sample_rows_into), CALL(rotary_into), CALL(logprobs_into), CALL(paged_attention_into), {nullptr, nullptr, 0, nullptr}};
+                           CALL(sample_rows_into), CALL(rotary_into), CALL(logprobs_into), CALL(paged_attention_into), CALL(paged_append_into), CALL(pool_rows_into), {nullptr, nullptr, 0, nullptr}};
 #undef CALL
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", "Operators of the C ABI without ctypes.", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -19,6 +19,7 @@
 #include "activation.cuh"
 #include "chain.cuh"
 #include "kernels.h"
+#include "kv_q4.cuh"
 
 namespace etc {
 
@@ -114,6 +115,7 @@ cudaError_t launch_kv_append(const PoolView& pool, const float* k, const float* 
                              const int* tables, int batch, int tokens, int64_t lane_stride, int64_t head_stride,
                              int64_t token_stride, cudaStream_t stream) {
   if (batch == 0 || tokens == 0) return cudaSuccess;
+  if (pool.dtype == kKvQ4) return launch_q4_append(pool, k, v, lanes, tables, batch, tokens, lane_stride, head_stride, token_stride, stream);
   dim3 grid((unsigned)tokens, (unsigned)pool.kv_heads, (unsigned)batch);
   const int threads = std::min(128, ((pool.head_dim + 31) / 32) * 32);
   kv_append_kernel<<<grid, threads, 0, stream>>>(pool, k, v, lanes, tables, lane_stride, head_stride, token_stride);
@@ -141,6 +143,18 @@ __device__ __forceinline__ float exact_load(const void* slab, size_t elem, float
   if (DTYPE == kKvF16) return __half2float(reinterpret_cast<const __half*>(slab)[elem]);
   if (DTYPE == kKvBF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(slab)[elem]);
   return __fmul_rn(__fsub_rn((float)reinterpret_cast<const uint8_t*>(slab)[elem], 128.0f), scale);
+}
+// Column c of a cached row (row = (page * kv_heads + head) * block_size + slot).
+template <int DTYPE>
+__device__ __forceinline__ float exact_value(const PoolView& p, bool is_v, int row, int c, float scale) {
+  void* slab = is_v ? p.v : p.k;
+  if constexpr (DTYPE == kKvQ4) {
+    const int record = row / p.block_size;  // pages of one head each
+    PoolView records = p;
+    records.kv_heads = 1;
+    return q4_value(q4_row(records, slab, record, 0, row - record * p.block_size), is_v, c, p.head_dim / 32);
+  }
+  return exact_load<DTYPE>(slab, (size_t)row * p.head_dim + c, scale);
 }
 
 // `tokens_first`: q and out are [B, tokens, Hq, D] (the fused projection's order) instead of [B, Hq, tokens, D].
@@ -189,18 +203,17 @@ __global__ void __launch_bounds__(128) attention_exact_kernel(PoolView pool, con
   for (int i = threadIdx.x; i < span; i += blockDim.x) {
     const int row = find_row(i);
     if (keep) row_of[i] = row;
-    const size_t base = (size_t)row * D;
     const float ks = k_scale(row);
     double score = 0.0;
     int c = 0;
     for (; c + 4 <= D; c += 4) {
       float kv[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) kv[u] = exact_load<DTYPE>(pool.k, base + c + u, ks);
+      for (int u = 0; u < 4; ++u) kv[u] = exact_value<DTYPE>(pool, false, row, c + u, ks);
 #pragma unroll
       for (int u = 0; u < 4; ++u) score += (double)q_s[c + u] * (double)kv[u];
     }
-    for (; c < D; ++c) score += (double)q_s[c] * (double)exact_load<DTYPE>(pool.k, base + c, ks);
+    for (; c < D; ++c) score += (double)q_s[c] * (double)exact_value<DTYPE>(pool, false, row, c, ks);
     const double scaled = __dmul_rn(score, scale);
     wrow[i] = scaled;
     local_max = fmax(local_max, scaled);
@@ -220,7 +233,7 @@ __global__ void __launch_bounds__(128) attention_exact_kernel(PoolView pool, con
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int row = row_at(i + u);
-        value[u] = exact_load<DTYPE>(pool.v, (size_t)row * D + c, v_scale(row));
+        value[u] = exact_value<DTYPE>(pool, true, row, c, v_scale(row));
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
@@ -232,7 +245,7 @@ __global__ void __launch_bounds__(128) attention_exact_kernel(PoolView pool, con
     for (; i < span; ++i) {
       const int row = row_at(i);
       const double w = wrow[i];
-      result = __dadd_rn(result, __dmul_rn(w, (double)exact_load<DTYPE>(pool.v, (size_t)row * D + c, v_scale(row))));
+      result = __dadd_rn(result, __dmul_rn(w, (double)exact_value<DTYPE>(pool, true, row, c, v_scale(row))));
       denominator = __dadd_rn(denominator, w);
     }
     orow[c] = (float)__ddiv_rn(result, denominator);
@@ -251,6 +264,7 @@ cudaError_t launch_attention_exact(const PoolView& pool, const float* q, const L
     case kKvF32: return launch(attention_exact_kernel<kKvF32>);
     case kKvF16: return launch(attention_exact_kernel<kKvF16>);
     case kKvBF16: return launch(attention_exact_kernel<kKvBF16>);
+    case kKvQ4: return launch(attention_exact_kernel<kKvQ4>);
     default: return launch(attention_exact_kernel<kKvU8>);
   }
 }
@@ -1505,22 +1519,31 @@ cudaError_t launch_record_step(const uint32_t* tokens, uint32_t* ids, uint32_t* 
 // Debug/test read-back of logical token rows (row = block*block_size + offset) as f32
 // [n, kv_heads*head_dim] in the reference's row order, dequantised for the u8 tier.
 __global__ void pool_read_rows_kernel(PoolView pool, const uint32_t* __restrict__ rows, int64_t n, float* __restrict__ out,
-                                      int which) {
+                                      int which, int64_t pool_rows, DeviceStatus* status) {
   const int64_t width = (int64_t)pool.kv_heads * pool.head_dim;
   const int64_t total = n * width;
   for (int64_t idx = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; idx < total; idx += (int64_t)gridDim.x * blockDim.x) {
     const int64_t i = idx / width, e = idx - i * width;
     const int head = (int)(e / pool.head_dim), d = (int)(e % pool.head_dim);
+    if (rows[i] >= pool_rows) {
+      if (atomicCAS(&status->code, kStatusNone, kStatusRowOutOfRange) == kStatusNone) {
+        status->value = rows[i];
+        status->bound = pool_rows;
+      }
+      out[idx] = 0.0f;
+      continue;
+    }
     const int page = (int)(rows[i] / pool.block_size), slot = (int)(rows[i] % pool.block_size);
     out[idx] = pool_load(pool, which == 0 ? pool.k : pool.v, which == 0 ? pool.k_scale : pool.v_scale,
                          pool_elem(pool, page, head, slot) + d, pool_scale_index(pool, page, head, slot));
   }
 }
-cudaError_t launch_pool_read_rows(const PoolView& pool, const uint32_t* rows, int64_t n, float* out, int which,
+cudaError_t launch_pool_read_rows(const PoolView& pool, const uint32_t* rows, int64_t n, float* out, int which, int64_t pool_rows, DeviceStatus* status,
                                   cudaStream_t stream) {
+  if (pool.dtype == kKvQ4) return launch_q4_rows(pool, rows, n, out, which, pool_rows, status, stream);
   const int64_t total = n * pool.kv_heads * pool.head_dim;
   if (total == 0) return cudaSuccess;
-  pool_read_rows_kernel<<<(unsigned)std::min<int64_t>((total + 255) / 256, 148 * 8), 256, 0, stream>>>(pool, rows, n, out, which);
+  pool_read_rows_kernel<<<(unsigned)std::min<int64_t>((total + 255) / 256, 148 * 8), 256, 0, stream>>>(pool, rows, n, out, which, pool_rows, status);
   return cudaGetLastError();
 }
 

@@ -43,7 +43,8 @@ struct DeviceStatus {
   long long reserved;
 };
 enum : unsigned long long {
-  kStatusNone = 0, kStatusIndexOutOfRange = 1, kStatusNonFiniteLogit = 2, kStatusTargetOutOfRange = 5, kStatusBadLogprobLogit = 6
+  kStatusNone = 0, kStatusIndexOutOfRange = 1, kStatusNonFiniteLogit = 2, kStatusTargetOutOfRange = 5, kStatusBadLogprobLogit = 6,
+  kStatusRowOutOfRange = 7
 };
 
 constexpr uint32_t kRuntimeMagic = 0x45544352;  // "ETCR"
@@ -88,5 +89,6 @@ const char* codec_name(int codec);
 int codec_block_values(int codec);
 int codec_block_bytes(int codec);
 int64_t codec_row_bytes(int codec, int64_t columns);  // -1 when invalid
-int kv_dtype_size(int dtype);
+// Bytes that `values` cached values of a tier take, without the u8 tier's scales; -1 for an unknown tier.
+int64_t kv_bytes(int dtype, int64_t values);
 }  // namespace etc

@@ -243,6 +243,7 @@ struct LaneInfo {
   int start;       // first position still resident (pool window), 0 without
   int table_offset;  // offset of this lane's block table in the tables array (index 0 = block of position 0)
 };
+constexpr int kKvQ4 = ETC_KV_Q4;
 cudaError_t launch_kv_append(const PoolView& pool, const float* k, const float* v, const LaneInfo* lanes,
                              const int* tables, int batch, int tokens, int64_t lane_stride, int64_t head_stride,
                              int64_t token_stride, cudaStream_t stream);
@@ -290,7 +291,25 @@ cudaError_t launch_rope_append(const PoolView& pool, const float* qkv, const Lan
 // them to the history, and advances every live lane's cursor (and window start) by one.
 cudaError_t launch_record_step(const uint32_t* tokens, uint32_t* ids, uint32_t* history, int* step_counter, LaneInfo* lanes,
                                int batch, long long window, cudaStream_t stream);
-cudaError_t launch_pool_read_rows(const PoolView& pool, const uint32_t* rows, int64_t n, float* out, int which,
+// Rows (page * block_size + slot, below pool_rows) of one slab as f32; others are reported through the status word and come out as zeros.
+cudaError_t launch_pool_read_rows(const PoolView& pool, const uint32_t* rows, int64_t n, float* out, int which, int64_t pool_rows, DeviceStatus* status,
                                   cudaStream_t stream);
+
+// ---- 4-bit pages (kv_q4.cu, attention_q4.cu) -------------------------------------------------
+cudaError_t launch_q4_append(const PoolView& pool, const float* k, const float* v, const LaneInfo* lanes, const int* tables, int batch, int tokens,
+                             int64_t lane_stride, int64_t head_stride, int64_t token_stride, cudaStream_t stream);
+cudaError_t launch_q4_rows(const PoolView& pool, const uint32_t* rows, int64_t n, float* out, int which, int64_t pool_rows, DeviceStatus* status,
+                           cudaStream_t stream);
+// One query token per lane; q and out [B, Hq, D] f32 (out_xh as launch_attention_mma's).
+struct Q4Plan {
+  int direct = 0;        // a CTA per (lane, KV head, group of query heads), no parts
+  int64_t ctas = 1;
+  size_t scratch_bytes = 0;
+};
+bool attention_q4_supported(const PoolView& pool, int q_heads);
+Q4Plan plan_attention_q4(int batch, int q_heads, int kv_heads, int head_dim, int max_pages, int sm_count);
+cudaError_t launch_attention_q4(const PoolView& pool, const float* q, const LaneInfo* lanes, const int* tables, int batch, int q_heads, double scale,
+                                long long op_window, float* out, const Q4Plan& plan, float* scratch, cudaStream_t stream, int* launches,
+                                __half* out_xh = nullptr, int xh_nv = 32);
 
 }  // namespace etc

@@ -1,0 +1,104 @@
+// The 4-bit KV tier: rows cut into blocks of 32 values with an f16 scale, by the Q4_0 rule (quant_kernels.cu): the value of largest
+// magnitude divided by -8 is the scale d, a code is floor(x / d + 8.5) held to 0..15 and stands for (code - 8) * d.
+//
+// One record per (page, KV head): the codes of its rows, head_dim / 2 bytes each, then their scales, head_dim / 32 f16 each; 18
+// bytes per block as in a GGUF row, and one contiguous run per page and head (1152 bytes for 16 rows of 128). Codes lie in a row so that
+// a thread of an m16n8k16 product finds its operands side by side (attention_q4.cu). With nb = head_dim / 32 blocks b:
+//   K: words [t][b], t < 4: elements 8 t .. 8 t + 7 of the block; even ones in the low half, odd ones in the high half, ascending
+//   V: half words [g][b], g < 8: elements g, g + 8, g + 16, g + 24 of the block, ascending
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "kernels.h"
+
+namespace etc {
+
+__host__ __device__ __forceinline__ size_t q4_record_bytes(int block_size, int head_dim) { return (size_t)block_size * (head_dim / 32) * 18; }
+
+struct Q4Row {
+  uint8_t* codes;
+  __half* scales;
+};
+__device__ __forceinline__ Q4Row q4_row(const PoolView& p, void* slab, int page, int head, int slot) {
+  uint8_t* record = reinterpret_cast<uint8_t*>(slab) + ((size_t)page * p.kv_heads + head) * q4_record_bytes(p.block_size, p.head_dim);
+  return {record + (size_t)slot * (p.head_dim / 2), reinterpret_cast<__half*>(record + (size_t)p.block_size * (p.head_dim / 2)) + (size_t)slot * (p.head_dim / 32)};
+}
+
+// One element, for the paths that are not in a hurry.
+__device__ __forceinline__ float q4_value(const Q4Row& row, bool is_v, int d, int nb) {
+  const int b = d >> 5, e = d & 31;
+  const int byte = is_v ? 2 * ((e & 7) * nb + b) + (e >> 4) : 4 * ((e >> 3) * nb + b) + 2 * (e & 1) + ((e >> 2) & 1);
+  const int shift = is_v ? (e & 8) >> 1 : (e & 2) << 1;
+  return __fmul_rn((float)(((row.codes[byte] >> shift) & 15) - 8), __half2float(row.scales[b]));
+}
+
+// Quantizes a block by four neighbouring lanes, lane t of which (the lowest two bits) holds elements 8 t .. 8 t + 7, and stores it where
+// `live`. All lanes of the warp take part; the four of a block agree on everything but the values.
+__device__ __forceinline__ void q4_store_block(const float (&v)[8], bool is_v, const Q4Row& row, int b, int nb, bool live) {
+  const int t = threadIdx.x & 3;
+  float extreme = 0.0f;  // a NaN is never taken
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (fabsf(v[i]) > fabsf(extreme)) extreme = v[i];
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) {
+    const float o = __shfl_xor_sync(0xffffffffu, extreme, off);
+    if (fabsf(o) > fabsf(extreme) || (fabsf(o) == fabsf(extreme) && (t & off))) extreme = o;  // of equals the first
+  }
+  const float d = __fmul_rn(extreme, -0.125f), inv = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
+  uint32_t code[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)  // the floor of a value in [0, 16) is the low byte of it plus 2^23, rounded down
+    code[i] = __float_as_uint(__fadd_rd(fminf(fmaxf(__fadd_rn(__fmul_rn(v[i], inv), 8.5f), 0.0f), 15.5f), 8388608.0f)) & 15u;
+  if (is_v) {
+    // element 8 t + g is code t of half word g: byte s of a lane's word holds its codes for g = 2 s and 2 s + 1
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mine |= code[i] << (4 * i);
+    uint32_t even = 0, odd = 0;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint32_t byte = __shfl_sync(0xffffffffu, mine, s, 4) >> (8 * t);
+      even |= (byte & 15u) << (4 * s);
+      odd |= ((byte >> 4) & 15u) << (4 * s);
+    }
+    if (live) {
+      uint16_t* dst = reinterpret_cast<uint16_t*>(row.codes);
+      dst[2 * t * nb + b] = (uint16_t)even;
+      dst[(2 * t + 1) * nb + b] = (uint16_t)odd;
+    }
+  } else if (live) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) word |= code[i] << (4 * (i >> 1) + 16 * (i & 1));
+    uint16_t* dst = reinterpret_cast<uint16_t*>(row.codes) + 2 * (t * nb + b);
+    if ((reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
+      *reinterpret_cast<uint32_t*>(dst) = word;
+    } else {  // pages of an odd number of blocks
+      dst[0] = (uint16_t)word;
+      dst[1] = (uint16_t)(word >> 16);
+    }
+  }
+  if (live && t == 0) row.scales[b] = __float2half_rn(d);
+}
+
+// The reverse: elements 8 t .. 8 t + 7 of block b.
+__device__ __forceinline__ void q4_load_block(const Q4Row& row, bool is_v, int b, int nb, bool live, float (&v)[8]) {
+  const int t = threadIdx.x & 3;
+  const uint16_t* src = reinterpret_cast<const uint16_t*>(row.codes);
+  const int at = is_v ? 2 * t * nb + b : 2 * (t * nb + b), next = is_v ? at + nb : at + 1;
+  const uint32_t word = live ? src[at] | (uint32_t)src[next] << 16 : 0u;
+  const float d = live ? __half2float(row.scales[b]) : 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint32_t code;
+    if (is_v) code = __shfl_sync(0xffffffffu, word, i >> 1, 4) >> (4 * t + 16 * (i & 1));
+    else code = word >> (4 * (i >> 1) + 16 * (i & 1));
+    v[i] = __fmul_rn((float)((int)(code & 15u) - 8), d);
+  }
+}
+
+}  // namespace etc

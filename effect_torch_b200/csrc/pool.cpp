@@ -173,9 +173,9 @@ using namespace etc;
 
 PoolView etc_pool::view(int layer) const {
   PoolView v;
-  const size_t esize = (size_t)kv_dtype_size(dtype);
-  v.k = (char*)d_k + (size_t)layer * layer_elems * esize;
-  v.v = (char*)d_v + (size_t)layer * layer_elems * esize;
+  const size_t layer_bytes = (size_t)kv_bytes(dtype, (int64_t)layer_elems);
+  v.k = (char*)d_k + (size_t)layer * layer_bytes;
+  v.v = (char*)d_v + (size_t)layer * layer_bytes;
   v.k_scale = d_k_scale ? d_k_scale + (size_t)layer * layer_scales : nullptr;
   v.v_scale = d_v_scale ? d_v_scale + (size_t)layer * layer_scales : nullptr;
   v.dtype = dtype;
@@ -235,8 +235,8 @@ etc_status etc_pool_create(etc_runtime* rt, int layers, int kv_heads, int head_d
   if (!out) return fail(ETC_INVALID_ARGUMENT, "out is null");
   *out = nullptr;
   // NativeKvPool::new geometry rules (napi/mod.rs:3651-3708)
-  if (dtype < ETC_KV_F32 || dtype > ETC_KV_U8)
-    return fail(ETC_INVALID_ARGUMENT, "kv pool: dtype must be f32, f16, bf16 or u8 (int8-quantized)");
+  if (dtype < ETC_KV_F32 || dtype > ETC_KV_Q4)
+    return fail(ETC_INVALID_ARGUMENT, "kv pool: dtype must be f32, f16, bf16, u8 (int8-quantized) or q4 (4-bit blocks)");
   if (layers < 0 || kv_heads < 0 || head_dim < 0) return fail(ETC_INVALID_ARGUMENT, "kv pool: negative geometry");
   if (layers == 0 && (kv_heads != 0 || head_dim != 0))
     return fail(ETC_INVALID_ARGUMENT, "kv pool: heads and head dim must be zero when layers is zero");
@@ -245,6 +245,8 @@ etc_status etc_pool_create(etc_runtime* rt, int layers, int kv_heads, int head_d
   if (block_size <= 0 || max_tokens <= 0 || max_tokens % block_size != 0)
     return fail(ETC_INVALID_ARGUMENT, "kv pool: capacity " + std::to_string(max_tokens) +
                                           " must be a positive multiple of block size " + std::to_string(block_size));
+  if (dtype == ETC_KV_Q4 && head_dim % 32 != 0)
+    return fail(ETC_INVALID_ARGUMENT, "kv pool: the q4 tier needs a head dim that is a multiple of 32, got " + std::to_string(head_dim));
   etc_pool* p = new etc_pool();
   static std::atomic<uint64_t> next_uid{1};
   p->uid = next_uid.fetch_add(1);
@@ -253,7 +255,7 @@ etc_status etc_pool_create(etc_runtime* rt, int layers, int kv_heads, int head_d
   p->max_tokens = max_tokens; p->block_size = block_size; p->dtype = dtype;
   p->layer_elems = (size_t)max_tokens * kv_heads * head_dim;
   p->layer_scales = (size_t)max_tokens * kv_heads;
-  const size_t bytes = p->layer_elems * layers * (size_t)kv_dtype_size(dtype);
+  const size_t bytes = (size_t)kv_bytes(dtype, (int64_t)p->layer_elems) * layers;
   etc_status st = rt->device_alloc(bytes, &p->d_k);
   if (st == ETC_OK) st = rt->device_alloc(bytes, &p->d_v);
   if (st == ETC_OK && dtype == ETC_KV_U8) {
@@ -305,9 +307,9 @@ etc_status etc_pool_stats(etc_pool* pool, uint32_t* capacity, uint32_t* free_blo
 
 etc_status etc_pool_state_bytes(int64_t layers, int64_t max_tokens, int64_t kv_heads, int64_t head_dim,
                                 etc_kv_dtype dtype, int64_t* out_bytes) {
-  const int size = kv_dtype_size(dtype);
-  if (size == 0) return fail(ETC_COMPILATION, "compile: unsupported KV state dtype");
-  int64_t bytes = layers * max_tokens * kv_heads * head_dim * 2 * size;
+  if (kv_bytes(dtype, 0) < 0) return fail(ETC_COMPILATION, "compile: unsupported KV state dtype");
+  if (dtype == ETC_KV_Q4 && head_dim % 32 != 0) return fail(ETC_COMPILATION, "compile: the q4 KV state needs a head dim that is a multiple of 32");
+  int64_t bytes = kv_bytes(dtype, layers * max_tokens * kv_heads * head_dim * 2);
   if (dtype == ETC_KV_U8) bytes += layers * max_tokens * kv_heads * 2 * 4;
   *out_bytes = bytes;
   return ETC_OK;
@@ -328,7 +330,7 @@ etc_status etc_pool_read_rows(etc_pool* pool, int layer, int which, const uint32
   uint32_t* d_rows = (uint32_t*)ws;
   float* d_out = (float*)((char*)ws + rows_bytes);
   ETC_CUDA(cudaMemcpyAsync(d_rows, h_rows, (size_t)n * sizeof(uint32_t), cudaMemcpyHostToDevice, rt->stream));
-  ETC_CUDA(launch_pool_read_rows(pool->view(layer), d_rows, n, d_out, which, rt->stream));
+  ETC_CUDA(launch_pool_read_rows(pool->view(layer), d_rows, n, d_out, which, pool->max_tokens, rt->d_status, rt->stream));
   rt->launches++;
   ETC_CUDA(cudaMemcpyAsync(h_out, d_out, (size_t)n * width * sizeof(float), cudaMemcpyDeviceToHost, rt->stream));
   ETC_CUDA(cudaStreamSynchronize(rt->stream));
@@ -475,6 +477,40 @@ etc_status stage_lanes(etc_runtime* rt, etc_pool* pool, int layer, etc_seq* cons
   return ETC_OK;
 }
 
+// Handles of the entry points that work on device-resident lanes and tables.
+etc_status check_paged(etc_runtime* rt, etc_pool* pool, int layer) {
+  if (!valid_pool(pool) || pool->rt != rt) return fail(ETC_INVALID_HANDLE, "kv pool belongs to a different runtime");
+  if (layer < 0 || layer >= pool->layers) return fail(ETC_INVALID_ARGUMENT, "kv attention: layer index out of range");
+  return ETC_OK;
+}
+
+etc_status check_decode_supported(const PoolView& view, int q_heads) {
+  if (view.dtype == ETC_KV_Q4 ? attention_q4_supported(view, q_heads) : attention_mma_supported(view, q_heads, 1)) return ETC_OK;
+  return fail(ETC_UNSUPPORTED, "kv attention: the tensor-core decode kernel needs an f16/bf16 pool with 16-token pages, head "
+                               "dim 64 or 128 and at most 16 query heads per kv head");
+}
+
+// Attention of one query token per lane, by the tier's kernel.
+etc_status decode_attention(etc_runtime* rt, const PoolView& view, const LaneInfo* d_lanes, const int* d_tables, int batch, int max_pages, const float* d_q,
+                            int q_heads, double scale, int64_t op_window, float* d_out, float* d_scratch, size_t scratch_bytes) {
+  auto check_scratch = [&](size_t needed) {
+    if (needed <= scratch_bytes && (needed == 0 || d_scratch)) return ETC_OK;
+    return fail(ETC_INVALID_ARGUMENT, "kv attention: scratch holds " + std::to_string(scratch_bytes) + " bytes, " + std::to_string(needed) + " needed");
+  };
+  int launches = 0;
+  if (view.dtype == ETC_KV_Q4) {
+    const Q4Plan plan = plan_attention_q4(batch, q_heads, view.kv_heads, view.head_dim, max_pages, rt->sm_count);
+    ETC_TRY(check_scratch(plan.scratch_bytes));
+    ETC_CUDA(launch_attention_q4(view, d_q, d_lanes, d_tables, batch, q_heads, scale, op_window, d_out, plan, d_scratch, rt->stream, &launches));
+  } else {
+    const AttnPlan plan = plan_attention(batch, q_heads, view.kv_heads, view.head_dim, max_pages, rt->sm_count);
+    ETC_TRY(check_scratch(plan.scratch_bytes));
+    ETC_CUDA(launch_attention_mma(view, d_q, d_lanes, d_tables, batch, q_heads, scale, op_window, d_out, plan, d_scratch, rt->stream, &launches));
+  }
+  rt->launches += (uint64_t)launches;
+  return ETC_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -524,11 +560,10 @@ etc_status etc_kv_attention_decode_into(etc_runtime* rt, etc_pool* pool, int lay
   if (pool->kv_heads == 0 || q_heads % pool->kv_heads != 0)
     return fail(ETC_EXECUTION, "kv attention: incompatible grouped-query q/k/v shapes");
   const PoolView view = pool->view(layer < pool->layers ? layer : 0);
-  if (!attention_mma_supported(view, q_heads, 1))
-    return fail(ETC_UNSUPPORTED, "kv attention: the tensor-core decode kernel needs an f16/bf16 pool with 16-token pages, head "
-                                 "dim 64 or 128 and at most 16 query heads per kv head");
-  const int D = pool->head_dim, Hkv = pool->kv_heads;
-  const size_t max_scratch = plan_attention_max_scratch(batch, q_heads, Hkv, D, pool->max_tokens / pool->block_size, rt->sm_count);
+  ETC_TRY(check_decode_supported(view, q_heads));
+  const int D = pool->head_dim, Hkv = pool->kv_heads, most_pages = pool->max_tokens / pool->block_size;
+  size_t max_scratch = plan_attention_max_scratch(batch, q_heads, Hkv, D, most_pages, rt->sm_count);
+  if (view.dtype == ETC_KV_Q4) max_scratch = plan_attention_q4(std::max(batch, 1), q_heads, Hkv, D, most_pages, rt->sm_count).scratch_bytes;
   StagedLanes st;
   ETC_TRY(stage_lanes(rt, pool, layer, seqs, batch, active, 1, 1, pool_window, 0, max_scratch + 256, &st));
   float* scratch = (float*)(((uintptr_t)st.d_extra + 255) & ~(uintptr_t)255);
@@ -536,11 +571,7 @@ etc_status etc_kv_attention_decode_into(etc_runtime* rt, etc_pool* pool, int lay
     ETC_CUDA(launch_kv_append(view, d_k, d_v, st.d_lanes, st.d_tables, batch, 1, (int64_t)Hkv * D, (int64_t)D, D, rt->stream));
     rt->launches++;
   }
-  const AttnPlan plan = plan_attention(batch, q_heads, Hkv, D, st.max_pages, rt->sm_count);
-  int launches = 0;
-  ETC_CUDA(launch_attention_mma(view, d_q, st.d_lanes, st.d_tables, batch, q_heads, scale, op_window, d_out, plan, scratch,
-                                rt->stream, &launches));
-  rt->launches += (uint64_t)launches;
+  ETC_TRY(decode_attention(rt, view, st.d_lanes, st.d_tables, batch, st.max_pages, d_q, q_heads, scale, op_window, d_out, scratch, max_scratch));
   ETC_CUDA(cudaStreamSynchronize(rt->stream));
   return ETC_OK;
 }
@@ -549,25 +580,53 @@ etc_status etc_paged_attention_into(etc_runtime* rt, etc_pool* pool, int layer, 
                                     int batch, int max_pages, const float* d_q, int q_heads, double scale, int64_t op_window,
                                     float* d_out, void* d_scratch, size_t scratch_bytes) {
   ETC_TRY(activate(rt));
-  if (!valid_pool(pool) || pool->rt != rt) return fail(ETC_INVALID_HANDLE, "kv pool belongs to a different runtime");
-  if (layer < 0 || layer >= pool->layers) return fail(ETC_INVALID_ARGUMENT, "kv attention: layer index out of range");
+  ETC_TRY(check_paged(rt, pool, layer));
   if (batch <= 0 || max_pages <= 0 || !d_lanes || !d_tables || !d_q || !d_out)
     return fail(ETC_INVALID_ARGUMENT, "kv attention: lanes, tables, q and out must be given for a positive batch and page bound");
   if (pool->kv_heads == 0 || q_heads % pool->kv_heads != 0)
     return fail(ETC_EXECUTION, "kv attention: incompatible grouped-query q/k/v shapes");
   const PoolView view = pool->view(layer);
-  if (!attention_mma_supported(view, q_heads, 1))
-    return fail(ETC_UNSUPPORTED, "kv attention: the tensor-core decode kernel needs an f16/bf16 pool with 16-token pages, head "
-                                 "dim 64 or 128 and at most 16 query heads per kv head");
+  ETC_TRY(check_decode_supported(view, q_heads));
   static_assert(sizeof(etc_lane) == sizeof(LaneInfo), "etc_lane is the kernel's lane descriptor");
-  const AttnPlan plan = plan_attention(batch, q_heads, pool->kv_heads, pool->head_dim, max_pages, rt->sm_count);
-  if (plan.scratch_bytes > scratch_bytes || (plan.scratch_bytes && !d_scratch))
-    return fail(ETC_INVALID_ARGUMENT, "kv attention: scratch holds " + std::to_string(scratch_bytes) + " bytes, " +
-                                          std::to_string(plan.scratch_bytes) + " needed");
-  int launches = 0;
-  ETC_CUDA(launch_attention_mma(view, d_q, reinterpret_cast<const LaneInfo*>(d_lanes), d_tables, batch, q_heads, scale, op_window,
-                                d_out, plan, reinterpret_cast<float*>(d_scratch), rt->stream, &launches));
-  rt->launches += (uint64_t)launches;
+  return decode_attention(rt, view, reinterpret_cast<const LaneInfo*>(d_lanes), d_tables, batch, max_pages, d_q, q_heads, scale, op_window, d_out,
+                          reinterpret_cast<float*>(d_scratch), scratch_bytes);
+}
+
+etc_status etc_paged_attention_scratch_bytes(etc_pool* pool, int batch, int q_heads, int max_pages, size_t* scratch_bytes) {
+  if (!valid_pool(pool)) return fail(ETC_INVALID_HANDLE, "kv pool handle is invalid or destroyed");
+  if (batch <= 0 || q_heads <= 0 || max_pages <= 0 || !scratch_bytes) return fail(ETC_INVALID_ARGUMENT, "kv attention plan: every argument must be positive");
+  if (pool->kv_heads == 0 || q_heads % pool->kv_heads != 0)
+    return fail(ETC_EXECUTION, "kv attention: incompatible grouped-query q/k/v shapes");
+  const PoolView view = pool->view(0);
+  ETC_TRY(check_decode_supported(view, q_heads));
+  const int sms = pool->rt->sm_count;
+  *scratch_bytes = view.dtype == ETC_KV_Q4 ? plan_attention_q4(batch, q_heads, view.kv_heads, view.head_dim, max_pages, sms).scratch_bytes
+                                           : plan_attention(batch, q_heads, view.kv_heads, view.head_dim, max_pages, sms).scratch_bytes;
+  return ETC_OK;
+}
+
+etc_status etc_paged_append_into(etc_runtime* rt, etc_pool* pool, int layer, const etc_lane* d_lanes, const int* d_tables, int batch, int tokens,
+                                 const float* d_k, const float* d_v) {
+  ETC_TRY(activate(rt));
+  ETC_TRY(check_paged(rt, pool, layer));
+  if (batch <= 0 || batch > 65535 || tokens <= 0 || !d_lanes || !d_tables || !d_k || !d_v)
+    return fail(ETC_INVALID_ARGUMENT, "kv append: lanes, tables, k and v must be given for a batch in 1..65535 of at least one token");
+  const int D = pool->head_dim, Hkv = pool->kv_heads;
+  ETC_CUDA(launch_kv_append(pool->view(layer), d_k, d_v, reinterpret_cast<const LaneInfo*>(d_lanes), d_tables, batch, tokens, (int64_t)Hkv * tokens * D,
+                            (int64_t)tokens * D, D, rt->stream));
+  rt->launches++;
+  return ETC_OK;
+}
+
+etc_status etc_pool_rows_into(etc_runtime* rt, etc_pool* pool, int layer, int which, const uint32_t* d_rows, int64_t n, float* d_out) {
+  ETC_TRY(activate(rt));
+  ETC_TRY(check_paged(rt, pool, layer));
+  if (which != 0 && which != 1) return fail(ETC_INVALID_ARGUMENT, "kv pool: which must be 0 (K) or 1 (V)");
+  if (n < 0 || n > INT32_MAX) return fail(ETC_INVALID_ARGUMENT, "kv pool: the number of rows must be in 0..2147483647");
+  if (n == 0) return ETC_OK;
+  if (!d_rows || !d_out) return fail(ETC_INVALID_ARGUMENT, "kv pool: rows and out must be device buffers");
+  ETC_CUDA(launch_pool_read_rows(pool->view(layer), d_rows, n, d_out, which, pool->max_tokens, rt->d_status, rt->stream));
+  rt->launches++;
   return ETC_OK;
 }
 

@@ -63,12 +63,13 @@ int64_t codec_row_bytes(int codec, int64_t columns) {
   if (values == 0 || columns < 0 || columns % values != 0) return -1;
   return columns / values * codec_block_bytes(codec);
 }
-int kv_dtype_size(int dtype) {
+int64_t kv_bytes(int dtype, int64_t values) {
   switch (dtype) {
-    case ETC_KV_F32: return 4;
-    case ETC_KV_F16: case ETC_KV_BF16: return 2;
-    case ETC_KV_U8: return 1;
-    default: return 0;
+    case ETC_KV_F32: return 4 * values;
+    case ETC_KV_F16: case ETC_KV_BF16: return 2 * values;
+    case ETC_KV_U8: return values;
+    case ETC_KV_Q4: return values / 32 * 18;
+    default: return -1;
   }
 }
 
@@ -138,6 +139,8 @@ etc_status etc_runtime::check_status() {
     return fail(ETC_EXECUTION, "sample: logit " + std::to_string(seen.value) + " is not finite");
   if (seen.code == 3) return fail(ETC_EXECUTION, "quantized_linear: a pipeline wait inside the kernel ran out; the launch gave up");
   if (seen.code == 4) return fail(ETC_EXECUTION, "tensor parallel: a peer never arrived at the all-reduce; the launch gave up");
+  if (seen.code == kStatusRowOutOfRange)
+    return fail(ETC_EXECUTION, "kv pool: row " + std::to_string(seen.value) + " is outside 0.." + std::to_string(seen.bound));
   if (seen.code == kStatusTargetOutOfRange)
     return fail(ETC_EXECUTION, "logprobs: target " + std::to_string(seen.value) + " is outside 0.." + std::to_string(seen.bound));
   if (seen.code == kStatusBadLogprobLogit)

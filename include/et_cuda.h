@@ -70,7 +70,12 @@ typedef enum etc_codec {
 } etc_codec;
 
 /* KV tiers (crates/runtime-cpu/src/pool.rs:20-25). */
-typedef enum etc_kv_dtype { ETC_KV_F32 = 0, ETC_KV_F16 = 1, ETC_KV_BF16 = 2, ETC_KV_U8 = 3 } etc_kv_dtype;
+typedef enum etc_kv_dtype {
+  ETC_KV_F32 = 0, ETC_KV_F16 = 1, ETC_KV_BF16 = 2, ETC_KV_U8 = 3,
+  /* 4 bits, added by this backend: blocks of 32 values along the head (head_dim a multiple of 32) under an f16 scale, quantized by the rule
+   * of etc_quantize_into for Q4_0; 18 bytes per block. A NaN takes no part in its block's scale and is stored as code 0. */
+  ETC_KV_Q4 = 4
+} etc_kv_dtype;
 
 /* RotaryLayout (crates/runtime-cpu/src/composed.rs:2714-2717). */
 typedef enum etc_rope_layout { ETC_ROPE_HALF_SPLIT = 0, ETC_ROPE_INTERLEAVED_PAIRS = 1 } etc_rope_layout;
@@ -476,12 +481,29 @@ ETC_API etc_status etc_peer_allreduce_into(etc_runtime* rt, int rank, int world,
  * graph and replayed. d_lanes[i] = {cursor, advance (1 = live lane, 0 = padded), start (first resident position),
  * table_offset (index in d_tables of the block that holds position 0)}; lane i attends over positions [start, cursor +
  * advance) (further narrowed by op_window). max_pages bounds the pages any lane attends over and fixes the split plan;
- * d_scratch holds etc_kv_attention_plan(...).partial_bytes for that plan. Needs an f16 / bf16 pool with 16-token pages. */
+ * d_scratch holds etc_paged_attention_scratch_bytes for that plan (of an f16, bf16 or u8 pool etc_kv_attention_plan(...).partial_bytes).
+ * Needs an f16, bf16, u8 or q4 pool with 16-token pages. Over a q4 pool nothing between the stored values and the result is rounded below
+ * f32; a lane may attend over no more than max_pages pages, as for the others. */
 typedef struct etc_lane { int cursor, advance, start, table_offset; } etc_lane;
 ETC_API etc_status etc_paged_attention_into(etc_runtime* rt, etc_pool* pool, int layer, const etc_lane* d_lanes,
                                             const int* d_tables, int batch, int max_pages, const float* d_q, int q_heads,
                                             double scale, int64_t op_window, float* d_out, void* d_scratch,
                                             size_t scratch_bytes);
+
+/* Scratch bytes that etc_paged_attention_into needs on this pool: the plan of the tier's kernel. f32 pools, and what else the decode
+ * kernels do not take, are refused as there. */
+ETC_API etc_status etc_paged_attention_scratch_bytes(etc_pool* pool, int batch, int q_heads, int max_pages, size_t* scratch_bytes);
+/* The scatter of etc_kv_append_into over device-resident lanes and block tables, any tier and page size, asynchronous and capturable
+ * like etc_paged_attention_into: rows 0 .. advance - 1 (at most `tokens`) of each lane go to positions cursor .. cursor + advance
+ * - 1, whose pages the tables must hold. d_k / d_v f32 [batch, kv_heads, tokens, head_dim]. A following
+ * etc_paged_attention_into with lanes {cursor + advance - 1, 1, start, table_offset} attends over them. */
+ETC_API etc_status etc_paged_append_into(etc_runtime* rt, etc_pool* pool, int layer, const etc_lane* d_lanes, const int* d_tables,
+                                         int batch, int tokens, const float* d_k, const float* d_v);
+/* etc_pool_read_rows on the device: the values that n rows of a layer's K (which 0) or V (1) slab stand for, f32 [n, kv_heads * head_dim]
+ * in d_out. d_rows holds row numbers (block * block_size + offset); one that the pool does not have comes out as zeros and is
+ * reported at the next synchronising call as ETC_EXECUTION "kv pool: row {r} is outside 0..{max_tokens}". Asynchronous, capturable. */
+ETC_API etc_status etc_pool_rows_into(etc_runtime* rt, etc_pool* pool, int layer, int which, const uint32_t* d_rows, int64_t n,
+                                      float* d_out);
 
 /* Planners of the flash-decoding kernel, pure host arithmetic in the manner of the reference's `*_requirements`
  * calls (crates/runtime-cpu/src/lib.rs:5-11). etc_kv_attention_plan: the split of `attended_pages` pages over the grid

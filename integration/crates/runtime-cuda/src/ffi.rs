@@ -38,6 +38,7 @@ pub const ETC_KV_F32: c_int = 0;
 pub const ETC_KV_F16: c_int = 1;
 pub const ETC_KV_BF16: c_int = 2;
 pub const ETC_KV_U8: c_int = 3;
+pub const ETC_KV_Q4: c_int = 4;
 
 /// `etc_rope_layout`, `etc_index_dtype`, `etc_epilogue`.
 pub const ETC_ROPE_HALF_SPLIT: c_int = 0;
@@ -552,6 +553,33 @@ extern "C" {
         d_out: *mut f32,
         d_scratch: *mut c_void,
         scratch_bytes: usize,
+    ) -> EtcStatus;
+    pub fn etc_paged_attention_scratch_bytes(
+        pool: *mut EtcPool,
+        batch: c_int,
+        q_heads: c_int,
+        max_pages: c_int,
+        scratch_bytes: *mut usize,
+    ) -> EtcStatus;
+    pub fn etc_paged_append_into(
+        rt: *mut EtcRuntime,
+        pool: *mut EtcPool,
+        layer: c_int,
+        d_lanes: *const EtcLane,
+        d_tables: *const c_int,
+        batch: c_int,
+        tokens: c_int,
+        d_k: *const f32,
+        d_v: *const f32,
+    ) -> EtcStatus;
+    pub fn etc_pool_rows_into(
+        rt: *mut EtcRuntime,
+        pool: *mut EtcPool,
+        layer: c_int,
+        which: c_int,
+        d_rows: *const u32,
+        n: i64,
+        d_out: *mut f32,
     ) -> EtcStatus;
     pub fn etc_kv_attention_plan(
         batch: c_int,
