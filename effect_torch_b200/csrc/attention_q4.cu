@@ -8,11 +8,13 @@
 // (22 bits together), after scaling by powers of two that keep the rest out of the subnormals; the products of both are added in f32.
 // Nothing else is below f32.
 //
-// Layout. Tokens are the rows of the first product and the columns of the second: S^T = K Q^T and O^T = V^T P^T. A group of four query
-// heads fills the eight columns of a tile with (value, rest) pairs, so the split costs no instructions of the tensor pipe as long as
-// four heads or fewer would leave columns empty anyway, and a thread's accumulators hold both parts of one head's scores, which it adds. A code
-// page is read from shared memory as it was stored: 16 bytes of a K row per thread are its operands of all eight steps, 8
-// bytes of a V row its operands of all eight tiles; two codes are widened by one mask and one f16 operation.
+// Layout. Tokens are the rows of the first product and the columns of the second: S^T = K Q^T and O^T = V^T P^T. A code page is read from
+// shared memory as it was stored: 16 bytes of a K row per thread are its operands of all eight steps, 8 bytes of a V row its operands of
+// all eight tiles; two codes are widened by one mask and one f16 operation. The eight columns of a tile are the heads of a KV head: up to
+// four (PAIRS) as (value, rest) pairs, so that the split costs no tensor instruction where columns would stay empty, and a thread
+// adds the two sums of its head; five to eight as they are, with a second product for the rests onto the same sums.
+//
+// What bounds it is the issue rate, not HBM: some 400 instructions per page and warp, 152 of them widening codes.
 //
 // Work. The pages of all (lane, KV head) units in a row are cut into as many equal runs as there are CTAs, whatever the lengths of the
 // lanes: no CTA waits for the longest. Warps take a run's pages in turn through a ring of cp.async copies that runs on across the
@@ -37,8 +39,10 @@ namespace {
 constexpr int kPage = 16;
 constexpr int kStages = 3;
 constexpr int kDirectPages = 16;
+constexpr int kUnitPages = 12;  // what a unit costs beyond its pages, in pages
+constexpr int kPartPad = 4;  // of a head's part: reference, sum of weights, two unused
 constexpr float kSlack = 6.0f;
-constexpr int kWeightBits = 8;  // weights p * dv / reference are scaled by 2^8: at most 2^14 with the slack
+constexpr float kWeightBits = 8.0f;  // weights are scaled by 2^8: at most 2^14 with the slack
 constexpr float kSmallestScale = 5.9604645e-8f;  // 2^-24, the smallest f16
 
 struct Q4Args {
@@ -50,7 +54,7 @@ struct Q4Args {
   float* out;      // [B, Hq, D]
   __half* out_xh;  // optional: in the hand-off layout
   int out_xh_nv;
-  float* partial;  // [CTAs][2][heads of a unit][D + 2]: O, then reference and sum of the weights
+  float* partial;  // [CTAs][2][heads of a unit][D + kPartPad]: O, then reference and sum of the weights
   int batch, q_heads, kv_heads;
   int groups, heads;  // query-head groups per KV head, heads of a group (the last may have fewer)
   int direct;
@@ -72,20 +76,23 @@ __device__ __forceinline__ Span span_of(const LaneInfo& info, long long op_windo
   return s;
 }
 
-// Pages of all lanes, by every warp for itself.
-__device__ __forceinline__ long long all_pages(const Q4Args& a) {
+// The work of all units lies in a row, lane by lane: a unit is kUnitPages places that stand for its start and end, then its pages.
+__device__ __forceinline__ int places_of(int pages) { return pages > 0 ? pages + kUnitPages : 0; }
+
+// Places of one unit of every lane, by every warp for itself.
+__device__ __forceinline__ long long all_places(const Q4Args& a) {
   long long sum = 0;
-  for (int i = threadIdx.x & 31; i < a.batch; i += 32) sum += span_of(a.lanes[i], a.op_window).pages;
+  for (int i = threadIdx.x & 31; i < a.batch; i += 32) sum += places_of(span_of(a.lanes[i], a.op_window).pages);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   return sum;
 }
-// The lane that holds the page `at` (of all lanes' pages times `units`), and how many pages times units come before it.
+// The lane that holds the place `at`, and how many places come before it.
 __device__ __forceinline__ void lane_at(const Q4Args& a, long long at, int units, int* found, long long* before) {
   long long base = 0;
   for (int i0 = 0; i0 < a.batch; i0 += 32) {
     const int i = i0 + (threadIdx.x & 31);
-    const long long mine = i < a.batch ? (long long)span_of(a.lanes[i], a.op_window).pages * units : 0;
+    const long long mine = i < a.batch ? (long long)places_of(span_of(a.lanes[i], a.op_window).pages) * units : 0;
     long long upto = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -105,13 +112,18 @@ __device__ __forceinline__ void lane_at(const Q4Args& a, long long at, int units
   *before = base;
 }
 
-__device__ __forceinline__ void copy16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+__device__ __forceinline__ void copy16(unsigned dst, const uint8_t* src) {  // dst in shared memory
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {  // onto zeros
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {  // of an 8 x 8 tile of f16 pairs
   uint32_t r;
@@ -125,12 +137,27 @@ __device__ __forceinline__ float exp2_flushed(float v) {
 }
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 halves(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-// Codes in bits 0-3 (LOW) or 4-7 of both halves of w -> two f16 numbers code - 8, exact: 1024 + code less 1032, or 1024 + 16 code over 16.
-template <bool LOW>
-__device__ __forceinline__ uint32_t widen(uint32_t w) {
-  if (LOW) return bits(__hsub2(halves((w & 0x000F000Fu) | 0x64006400u), __floats2half2_rn(1032.0f, 1032.0f)));
-  return bits(__hfma2(halves((w & 0x00F000F0u) | 0x64006400u), __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-72.0f, -72.0f)));
-}
+// Constants of the widening, each in a register of its own: as immediates they would cost an instruction more per use.
+struct Widen {
+  uint32_t exponent, bias, sixteenth, shift;
+  __device__ __forceinline__ Widen() {
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(exponent));   // 1024 in both halves
+    asm volatile("mov.b32 %0, 0xE408E408;" : "=r"(bias));       // -1032
+    asm volatile("mov.b32 %0, 0x2C002C00;" : "=r"(sixteenth));  // 1 / 16
+    asm volatile("mov.b32 %0, 0xD480D480;" : "=r"(shift));      // -72
+  }
+  // Codes in bits 0-3 (LOW) or 4-7 of both halves of w -> two f16 numbers code - 8, exact: 1024 + code less 1032, or 1024 + 16 code over 16.
+  template <bool LOW>
+  __device__ __forceinline__ uint32_t get(uint32_t w) const {
+    uint32_t r;
+    if (LOW) {
+      asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(r) : "r"(w), "r"(exponent));
+      return bits(__hadd2(halves(r), halves(bias)));
+    }
+    asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(r) : "r"(w), "r"(exponent));
+    return bits(__hfma2(halves(r), halves(sixteenth), halves(shift)));
+  }
+};
 // 2^k with |x| 2^k in [2^13, 2^14), for a finite x that is not 0; 1 otherwise.
 __device__ __forceinline__ float to_f16_range(float x) {
   const int e = (int)((__float_as_uint(x) >> 23) & 255u);
@@ -138,31 +165,42 @@ __device__ __forceinline__ float to_f16_range(float x) {
   return __uint_as_float((unsigned)min(max(127 + 13 - (e - 127), 1), 254) << 23);
 }
 
-template <int D, int NT, int WARPS>
+// What V scales are multiplied by, of which no |dv| exceeds the power of two `top`: 1 / top, as far as f16 holds it.
+__device__ __forceinline__ __half2 scale_to_range(float top) { return __float2half2_rn(fminf(1.0f / top, 32768.0f)); }
+
+template <int D, bool PAIRS, int WARPS>
 struct Q4Cfg {
   static constexpr int kBlocks = D / 32;
   static constexpr int kCodes = kPage * D / 2;                  // code bytes of a record
   static constexpr int kRecord = kCodes + kPage * kBlocks * 2;
   static constexpr int kStage = 2 * kRecord;                    // K, then V
-  static constexpr int kHeads = 4 * NT;
+  static constexpr int kHeads = PAIRS ? 4 : 8;
   static constexpr int kPitch = D + 8;                          // of a head's partial sums: no bank conflicts
   static constexpr int kRing = WARPS * kStages * kStage;
   static constexpr size_t kSmem = kRing + (size_t)WARPS * kHeads * (kPitch + 2) * sizeof(float);
 };
 
+// N words (1, 2 or 4) from shared memory, aligned to their size.
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t* dst, const unsigned char* src) {
+  if constexpr (N == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+  else if constexpr (N == 2) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
+  else dst[0] = *reinterpret_cast<const uint32_t*>(src);
+}
+
 // A run of work, page by page for one warp: the unit it is in and its next page there.
 struct Cursor {
-  long long at, stop;  // position of the current unit's first page of this run in the row of all pages, and the run's end
+  long long at, stop;  // the places where the unit, or the run, ends
   int lane, unit;      // unit: KV head * groups + group
   Span span;
   int table;
   int page0, page1;    // this run's pages of the unit (block-table indexes)
 };
 
-template <int D, int NT, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 16 / WARPS : 12 / WARPS) attention_q4_kernel(Q4Args a) {
-  using Cfg = Q4Cfg<D, NT, WARPS>;
-  constexpr int NB = Cfg::kBlocks;
+template <int D, bool PAIRS, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) attention_q4_kernel(Q4Args a) {
+  using Cfg = Q4Cfg<D, PAIRS, WARPS>;
+  constexpr int NB = Cfg::kBlocks, MINE = PAIRS ? 1 : 2;  // heads whose scores a thread holds: t, or 2 t and 2 t + 1
   extern __shared__ __align__(128) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int units = a.kv_heads * a.groups, G = a.q_heads / a.kv_heads;
@@ -175,36 +213,36 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 16 / WARPS : 12 / WARPS)
     c.span = span_of(info, a.op_window);
     c.table = info.table_offset;
   };
+  // the part of the unit from its place `skipped` on; it may hold no page
   auto clip = [&](Cursor& c, int skipped) {
-    c.page0 = c.span.first + skipped;
-    c.page1 = c.span.first + (int)min((long long)c.span.pages, skipped + (c.stop - c.at));
+    const int places = c.span.pages + kUnitPages, upto = (int)min((long long)places, skipped + (c.stop - c.at));
+    c.page0 = c.span.first + max(skipped - kUnitPages, 0);
+    c.page1 = c.span.first + max(upto - kUnitPages, 0);
+    c.at += upto - skipped;  // where the next unit begins
   };
-  // the next unit of the run; false when it is done
+  // the next unit of the run of which it has pages; false when there is none
   auto advance = [&](Cursor& c) {
-    c.at += c.page1 - c.page0;
-    if (c.at >= c.stop) return false;
-    if (++c.unit == units) {
-      c.unit = 0;
-      do ++c.lane; while (c.lane < a.batch && span_of(a.lanes[c.lane], a.op_window).pages == 0);
-      if (c.lane >= a.batch) return false;
-      enter(c);
+    while (c.at < c.stop) {
+      if (++c.unit == units) {
+        c.unit = 0;
+        do ++c.lane; while (c.lane < a.batch && span_of(a.lanes[c.lane], a.op_window).pages == 0);
+        if (c.lane >= a.batch) return false;
+        enter(c);
+      }
+      clip(c, 0);
+      if (c.page0 < c.page1) return true;
     }
-    clip(c, 0);
-    return true;
+    return false;
   };
   if (a.direct) {
     run.lane = blockIdx.x / units;
     run.unit = blockIdx.x - run.lane * units;
     run.at = 0;
     enter(run);
-    run.stop = run.span.pages;
-    if (run.stop == 0) {
-      run.page0 = run.page1 = 0;
-    } else {
-      clip(run, 0);
-    }
+    run.stop = places_of(run.span.pages);
+    clip(run, 0);
   } else {
-    const long long total = all_pages(a) * units;
+    const long long total = all_places(a) * units;
     const long long begin = total * blockIdx.x / gridDim.x;
     run.stop = total * (blockIdx.x + 1) / gridDim.x;
     if (begin >= run.stop) return;
@@ -213,53 +251,76 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 16 / WARPS : 12 / WARPS)
     enter(run);
     run.at = begin;
     const long long inside = begin - before;
-    run.unit = (int)(inside / run.span.pages);
-    clip(run, (int)(inside - (long long)run.unit * run.span.pages));
+    const int places = places_of(run.span.pages);
+    run.unit = (int)(inside / places);
+    clip(run, (int)(inside - (long long)run.unit * places));
+    if (run.page0 == run.page1 && !advance(run)) return;
   }
   const bool idle = run.page0 == run.page1;  // direct: a lane with nothing to attend over
 
-  // the ring: this warp's pages, from `ahead`, the cursor that copies are issued from
+  // the ring: this warp's pages, from `ahead`, the cursor that copies are issued from; the number of the page that comes next is
+  // looked up one copy ahead
   unsigned char* ring = smem + warp * (kStages * Cfg::kStage);
+  const unsigned ring_at = (unsigned)__cvta_generic_to_shared(ring) + lane * 16;
   Cursor ahead = run;
-  int ahead_page = idle ? 0 : run.page0 + warp;
+  int ahead_page = run.page0 + warp;
+  unsigned ahead_number = 0;
+  const uint8_t *ahead_k, *ahead_v;  // page 0 of the unit's KV head, this lane's 16 bytes
   bool more = !idle;
-  const size_t page_stride = (size_t)a.kv_heads * Cfg::kRecord;
-  auto issue = [&](int stage) {
+  const unsigned page_stride = (unsigned)(a.kv_heads * Cfg::kRecord);
+  auto aim = [&] {
+    const size_t from = (size_t)(ahead.unit / a.groups) * Cfg::kRecord + lane * 16;
+    ahead_k = a.k + from;
+    ahead_v = a.v + from;
+  };
+  auto look_up = [&] {
     while (more && ahead_page >= ahead.page1) {
       more = advance(ahead);
       ahead_page = ahead.page0 + warp;
+      aim();
     }
+    if (more) ahead_number = (unsigned)a.tables[ahead.table + ahead_page];
+  };
+  aim();
+  look_up();
+  auto issue = [&](unsigned offset) {
     if (more) {
-      const size_t off = (size_t)a.tables[ahead.table + ahead_page] * page_stride + (size_t)(ahead.unit / a.groups) * Cfg::kRecord;
-      unsigned char* dst = ring + stage * Cfg::kStage;
+      const uint8_t *k = ahead_k + (unsigned long long)ahead_number * page_stride, *v = ahead_v + (unsigned long long)ahead_number * page_stride;
+      const unsigned dst = ring_at + offset;
 #pragma unroll
-      for (int c = lane; c < Cfg::kRecord / 16; c += 32) {
-        copy16(dst + c * 16, a.k + off + c * 16);
-        copy16(dst + Cfg::kRecord + c * 16, a.v + off + c * 16);
-      }
+      for (int c = 0; c < Cfg::kRecord; c += 512)
+        if (c + 512 <= Cfg::kRecord || lane * 16 + c < Cfg::kRecord) {
+          copy16(dst + c, k + c);
+          copy16(dst + Cfg::kRecord + c, v + c);
+        }
       ahead_page += WARPS;
+      look_up();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  unsigned fill = 0, at = 0;  // ring offsets of the next copy and of the page at hand
+  auto step = [](unsigned& offset) { offset = offset == (kStages - 1) * Cfg::kStage ? 0 : offset + Cfg::kStage; };
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) issue(s);
+  for (int s = 0; s < kStages - 1; ++s) {
+    issue(fill);
+    step(fill);
+  }
 
   float* sums = reinterpret_cast<float*>(smem + Cfg::kRing);  // [warp][head][pitch], then references and weights [warp][head]
   float* refs = sums + WARPS * Cfg::kHeads * Cfg::kPitch;
   float* weights = refs + WARPS * Cfg::kHeads;
-  const int row_lo = (g >> 1) + 4 * (g & 1), row_hi = row_lo + 8;  // tokens of this thread's scores: row r of a tile is token r/2 + 4 (r%2)
+  const int row_lo = (g >> 1) + 4 * (g & 1);  // tokens of this thread's scores, row_lo and row_lo + 8: row r of a tile is token r/2 + 4 (r%2)
+  const Widen widen;
   const bool wide_q = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;
-  int stage = 0;
   bool first_unit = true;
   while (true) {
     const int kv_head = run.unit / a.groups, head0 = kv_head * G + (run.unit - kv_head * a.groups) * a.heads;
     const int live_heads = min(a.heads, (kv_head + 1) * G - head0);
-    // queries: column g of tile n is the value (g even) or the rest (g odd) of head 4 n + g / 2
-    uint32_t qf[NT][NB][2][2];
-    float unscale[NT];  // of the scores of head 4 n + t
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int h = 4 * n + (g >> 1);
+    // queries: column g is the value (g even) or the rest (g odd) of head g / 2, or value and rest, one after the other, of head g
+    uint32_t qf[PAIRS ? 1 : 2][NB][2][2];
+    float unscale[MINE];
+    {
+      const int h = PAIRS ? g >> 1 : g;
       const bool live = h < live_heads;
       const float* q = a.q + ((size_t)run.lane * a.q_heads + head0 + (live ? h : 0)) * D + 8 * t;
       float4 x[NB][2];
@@ -276,195 +337,223 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 16 / WARPS : 12 / WARPS)
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
       const float f = to_f16_range(most);
-      unscale[n] = __shfl_sync(0xffffffffu, a.scale_log2 / f, 8 * t);
-      auto split = [&](float u, float v) {
-        u *= f;
-        v *= f;
-        const __half2 value = __floats2half2_rn(u, v);
-        if ((g & 1) == 0) return bits(value);
-        return bits(__floats2half2_rn(u - __low2float(value), v - __high2float(value)));
-      };
+#pragma unroll
+      for (int m = 0; m < MINE; ++m) unscale[m] = __shfl_sync(0xffffffffu, a.scale_log2 / f, PAIRS ? 8 * t : 4 * (2 * t + m));
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          qf[n][b][s][0] = split(x[b][s].x, x[b][s].y);
-          qf[n][b][s][1] = split(x[b][s].z, x[b][s].w);
-        }
-    }
-    float o[NT][2 * NB][4];
-    float ref[NT], weight[NT];  // of head 4 n + t; the sum of weights is this thread's share
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      ref[n] = -INFINITY;
-      weight[n] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 2 * NB; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+          for (int p = 0; p < 2; ++p) {
+            const float u = f * (p ? x[b][s].z : x[b][s].x), v = f * (p ? x[b][s].w : x[b][s].y);
+            const __half2 value = __floats2half2_rn(u, v), rest = __floats2half2_rn(u - __low2float(value), v - __high2float(value));
+            if constexpr (PAIRS) {
+              qf[0][b][s][p] = (g & 1) == 0 ? bits(value) : bits(rest);
+            } else {
+              qf[0][b][s][p] = bits(value);
+              qf[1][b][s][p] = bits(rest);
+            }
+          }
     }
+    float o[2 * NB][4];
+    float ref[MINE], limit[MINE], sub[MINE], weight[MINE];  // reference, score that raises it, what weights' exponents are less, this thread's sum of weights
+#pragma unroll
+    for (int m = 0; m < MINE; ++m) {
+      ref[m] = limit[m] = -INFINITY;
+      sub[m] = -kWeightBits;  // for as long as every score is -inf or NaN
+      weight[m] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
     float top_scale = kSmallestScale;  // power of two that no |dv| so far exceeds
+    __half2 top_half = __float2half2_rn(top_scale), to_range = scale_to_range(top_scale);
+    const int inner0 = (run.span.begin + kPage - 1) / kPage, inner1 = run.span.end / kPage;  // pages without a masked token
 
     for (int page = run.page0 + warp; page < run.page1; page += WARPS) {
-      issue((stage + kStages - 1) % kStages);
+      issue(fill);
+      step(fill);
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       __syncwarp();
-      const unsigned char* ks = ring + stage * Cfg::kStage;
-      const unsigned char* vs = ks + Cfg::kRecord;
-      const bool live_lo = page * kPage + row_lo >= run.span.begin && page * kPage + row_lo < run.span.end;
-      const bool live_hi = page * kPage + row_hi >= run.span.begin && page * kPage + row_hi < run.span.end;
+      const unsigned char *codes = ring + at + row_lo * (D / 2) + t * (4 * NB), *scales = ring + at + Cfg::kCodes + row_lo * (2 * NB);
 
       // scores of tokens row_lo and row_hi
-      float s_lo[NT], s_hi[NT];
+      float s_lo[MINE], s_hi[MINE];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s_lo[n] = s_hi[n] = 0.0f;
+      for (int m = 0; m < MINE; ++m) s_lo[m] = s_hi[m] = 0.0f;
       {
         __align__(16) uint32_t w_lo[NB], w_hi[NB];
         __align__(8) uint32_t d_lo[NB / 2], d_hi[NB / 2];
-        const unsigned char *lo = ks + row_lo * (D / 2) + t * (4 * NB), *hi = ks + row_hi * (D / 2) + t * (4 * NB);
-        const unsigned char *scale_lo = ks + Cfg::kCodes + row_lo * (2 * NB), *scale_hi = ks + Cfg::kCodes + row_hi * (2 * NB);
-        if constexpr (NB == 4) {
-          *reinterpret_cast<uint4*>(w_lo) = *reinterpret_cast<const uint4*>(lo);
-          *reinterpret_cast<uint4*>(w_hi) = *reinterpret_cast<const uint4*>(hi);
-          *reinterpret_cast<uint2*>(d_lo) = *reinterpret_cast<const uint2*>(scale_lo);
-          *reinterpret_cast<uint2*>(d_hi) = *reinterpret_cast<const uint2*>(scale_hi);
-        } else {
-          *reinterpret_cast<uint2*>(w_lo) = *reinterpret_cast<const uint2*>(lo);
-          *reinterpret_cast<uint2*>(w_hi) = *reinterpret_cast<const uint2*>(hi);
-          d_lo[0] = *reinterpret_cast<const uint32_t*>(scale_lo);
-          d_hi[0] = *reinterpret_cast<const uint32_t*>(scale_hi);
-        }
+        load_words<NB>(w_lo, codes);
+        load_words<NB>(w_hi, codes + 8 * (D / 2));
+        load_words<NB / 2>(d_lo, scales);
+        load_words<NB / 2>(d_hi, scales + 8 * (2 * NB));
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           const uint32_t x = w_lo[b], y = w_hi[b], x8 = x >> 8, y8 = y >> 8;
-          const uint32_t a00 = widen<true>(x), a01 = widen<true>(y), a02 = widen<false>(x), a03 = widen<false>(y);
-          const uint32_t a10 = widen<true>(x8), a11 = widen<true>(y8), a12 = widen<false>(x8), a13 = widen<false>(y8);
+          const uint32_t a00 = widen.get<true>(x), a01 = widen.get<true>(y), a02 = widen.get<false>(x), a03 = widen.get<false>(y);
+          const uint32_t a10 = widen.get<true>(x8), a11 = widen.get<true>(y8), a12 = widen.get<false>(x8), a13 = widen.get<false>(y8);
           const float2 dl = __half22float2(halves(d_lo[b / 2])), dh = __half22float2(halves(d_hi[b / 2]));
+          const float d0 = b & 1 ? dl.y : dl.x, d1 = b & 1 ? dh.y : dh.x;
+          float c[4];
+          mma_first(c, a00, a01, a02, a03, qf[0][b][0][0], qf[0][b][0][1]);
+          mma(c, a10, a11, a12, a13, qf[0][b][1][0], qf[0][b][1][1]);
+          if constexpr (PAIRS) {
+            s_lo[0] = fmaf(d0, c[0] + c[1], s_lo[0]);
+            s_hi[0] = fmaf(d1, c[2] + c[3], s_hi[0]);
+          } else {
+            mma(c, a00, a01, a02, a03, qf[1][b][0][0], qf[1][b][0][1]);
+            mma(c, a10, a11, a12, a13, qf[1][b][1][0], qf[1][b][1][1]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-            mma(c, a00, a01, a02, a03, qf[n][b][0][0], qf[n][b][0][1]);
-            mma(c, a10, a11, a12, a13, qf[n][b][1][0], qf[n][b][1][1]);
-            s_lo[n] = fmaf(b & 1 ? dl.y : dl.x, c[0] + c[1], s_lo[n]);
-            s_hi[n] = fmaf(b & 1 ? dh.y : dh.x, c[2] + c[3], s_hi[n]);
+            for (int m = 0; m < MINE; ++m) {
+              s_lo[m] = fmaf(d0, c[m], s_lo[m]);
+              s_hi[m] = fmaf(d1, c[2 + m], s_hi[m]);
+            }
           }
         }
       }
       __align__(8) uint32_t dv_lo[NB / 2], dv_hi[NB / 2];
-      {
-        const unsigned char *scale_lo = vs + Cfg::kCodes + row_lo * (2 * NB), *scale_hi = vs + Cfg::kCodes + row_hi * (2 * NB);
-        if constexpr (NB == 4) {
-          *reinterpret_cast<uint2*>(dv_lo) = *reinterpret_cast<const uint2*>(scale_lo);
-          *reinterpret_cast<uint2*>(dv_hi) = *reinterpret_cast<const uint2*>(scale_hi);
-        } else {
-          dv_lo[0] = *reinterpret_cast<const uint32_t*>(scale_lo);
-          dv_hi[0] = *reinterpret_cast<const uint32_t*>(scale_hi);
+      load_words<NB / 2>(dv_lo, scales + Cfg::kRecord);
+      load_words<NB / 2>(dv_hi, scales + Cfg::kRecord + 8 * (2 * NB));
+#pragma unroll
+      for (int m = 0; m < MINE; ++m) {
+        s_lo[m] *= unscale[m];
+        s_hi[m] *= unscale[m];
+      }
+      if (page < inner0 || page >= inner1) {
+        // a masked token's rows may hold anything: neither its score nor its scales are looked at
+        const int pos_lo = page * kPage + row_lo, pos_hi = pos_lo + 8;
+        const bool live_lo = pos_lo >= run.span.begin && pos_lo < run.span.end, live_hi = pos_hi >= run.span.begin && pos_hi < run.span.end;
+#pragma unroll
+        for (int m = 0; m < MINE; ++m) {
+          if (!live_lo) s_lo[m] = -INFINITY;
+          if (!live_hi) s_hi[m] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < NB / 2; ++i) {
+          if (!live_lo) dv_lo[i] = 0u;
+          if (!live_hi) dv_hi[i] = 0u;
         }
       }
-      // a masked token's rows may hold anything: neither its score nor its scale is looked at
-      bool rises = false;
+      __half2 largest = __hmax2(__habs2(halves(dv_lo[0])), __habs2(halves(dv_hi[0])));
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        s_lo[n] = live_lo ? s_lo[n] * unscale[n] : -INFINITY;
-        s_hi[n] = live_hi ? s_hi[n] * unscale[n] : -INFINITY;
-        rises = rises || !(s_lo[n] <= ref[n] + kSlack) || !(s_hi[n] <= ref[n] + kSlack);
-      }
-      __half2 largest = __float2half2_rn(0.0f);
+      for (int i = 1; i < NB / 2; ++i) largest = __hmax2(largest, __hmax2(__habs2(halves(dv_lo[i])), __habs2(halves(dv_hi[i]))));
+      bool rises = !__hble2(largest, top_half);
 #pragma unroll
-      for (int i = 0; i < NB / 2; ++i) {
-        if (!live_lo) dv_lo[i] = 0u;
-        if (!live_hi) dv_hi[i] = 0u;
-        largest = __hmax2(largest, __hmax2(__habs2(halves(dv_lo[i])), __habs2(halves(dv_hi[i]))));
-      }
-      // an infinite scale spoils its own columns only: the reference stays finite
-      const float largest_scale = fminf(fmaxf(__low2float(largest), __high2float(largest)), 65504.0f);
-      rises = rises || largest_scale > top_scale;
+      for (int m = 0; m < MINE; ++m) rises = rises || !(s_lo[m] <= limit[m]) || !(s_hi[m] <= limit[m]);
       if (__any_sync(0xffffffffu, rises)) {
-        float scale = largest_scale;
+        // an infinite scale spoils its own columns only: the reference stays finite
+        float scale = fminf(fmaxf(__low2float(largest), __high2float(largest)), 65504.0f), shrink = 1.0f;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) scale = fmaxf(scale, __shfl_xor_sync(0xffffffffu, scale, off));
-        float shrink = 1.0f;
         if (scale > top_scale) {
-          const float raised = __uint_as_float((__float_as_uint(scale) + 0x7fffffu) & 0x7f800000u);  // the power of two at or above it
-          shrink = top_scale / raised;
-          top_scale = raised;
+          top_scale = __uint_as_float((__float_as_uint(scale) + 0x7fffffu) & 0x7f800000u);  // the power of two at or above it
+          top_half = __float2half2_rn(top_scale);
+          const __half2 range = scale_to_range(top_scale);
+          shrink = __low2float(range) / __low2float(to_range);
+          to_range = range;
         }
+        float f[MINE];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float most = fmaxf(s_lo[n], s_hi[n]);
+        for (int m = 0; m < MINE; ++m) {
+          float most = fmaxf(s_lo[m], s_hi[m]);
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-          float f = 1.0f;
-          if (most > ref[n] + kSlack) {  // each head for itself: its result does not depend on the others
-            f = exp2_flushed(ref[n] - most);
-            ref[n] = most;
+          f[m] = 1.0f;
+          if (most > limit[m]) {  // each head for itself: its result does not depend on the others
+            f[m] = exp2_flushed(ref[m] - most);
+            ref[m] = most;
+            limit[m] = most + kSlack;
+            sub[m] = most - kWeightBits;
           }
-          weight[n] *= f;
-          f *= shrink;
+          weight[m] *= f[m];
+          f[m] *= shrink;
+        }
 #pragma unroll
-          for (int i = 0; i < 2 * NB; ++i) {
-            o[n][i][0] *= f; o[n][i][1] *= f; o[n][i][2] *= f; o[n][i][3] *= f;
-          }
+        for (int i = 0; i < 2 * NB; ++i) {
+          o[i][0] *= f[0]; o[i][1] *= f[MINE - 1]; o[i][2] *= f[0]; o[i][3] *= f[MINE - 1];
         }
       }
-      // weights, and their products with the V scales as (value, rest) pairs, transposed into operand order
-      uint32_t pf[NT][NB][2];
-      const float to_range = (float)(1 << kWeightBits) / top_scale;
+      // Weights, and their products with the V scales as value and rest, transposed into operand order. All in f16: w is the weight's value
+      // and x its rest, w * d rounds to the product's value, and fma gives what that leaves out exactly, to which x * d is added.
+      uint32_t pf[PAIRS ? 1 : 2][NB][2];
+      float p_lo[MINE], p_hi[MINE];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float sub = ref[n] == -INFINITY ? 0.0f : ref[n];
-        float p_lo = exp2_flushed(s_lo[n] - sub), p_hi = exp2_flushed(s_hi[n] - sub);
-        weight[n] += p_lo + p_hi;
-        p_lo *= to_range;
-        p_hi *= to_range;
+      for (int m = 0; m < MINE; ++m) {
+        p_lo[m] = exp2_flushed(s_lo[m] - sub[m]);
+        p_hi[m] = exp2_flushed(s_hi[m] - sub[m]);
+        weight[m] += p_lo[m] + p_hi[m];
+      }
+      auto product = [](__half2 w, __half2 x, __half2 d, __half2& value, __half2& rest) {
+        value = __hmul2(w, d);
+        rest = __hfma2(x, d, __hfma2(w, d, __hneg2(value)));
+      };
+      auto rest_of = [](float u, float v, __half2 value) { return __floats2half2_rn(u - __low2float(value), v - __high2float(value)); };
+      if constexpr (PAIRS) {
+        const __half2 w = __floats2half2_rn(p_lo[0], p_hi[0]), x = rest_of(p_lo[0], p_hi[0], w);
+        const __half2 w_lo = __low2half2(w), w_hi = __high2half2(w), x_lo = __low2half2(x), x_hi = __high2half2(x);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const float2 dl = __half22float2(halves(dv_lo[b / 2])), dh = __half22float2(halves(dv_hi[b / 2]));
-          const float w_lo = p_lo * (b & 1 ? dl.y : dl.x), w_hi = p_hi * (b & 1 ? dh.y : dh.x);
-          const __half2 value = __floats2half2_rn(w_lo, w_hi);
-          const __half2 rest = __floats2half2_rn(w_lo - __low2float(value), w_hi - __high2float(value));
-          pf[n][b][0] = transpose8(bits(__lows2half2(value, rest)));
-          pf[n][b][1] = transpose8(bits(__highs2half2(value, rest)));
+        for (int i = 0; i < NB / 2; ++i) {  // two blocks at a time
+          __half2 value_lo, rest_lo, value_hi, rest_hi;
+          product(w_lo, x_lo, __hmul2(halves(dv_lo[i]), to_range), value_lo, rest_lo);
+          product(w_hi, x_hi, __hmul2(halves(dv_hi[i]), to_range), value_hi, rest_hi);
+          pf[0][2 * i][0] = transpose8(bits(__lows2half2(value_lo, rest_lo)));
+          pf[0][2 * i][1] = transpose8(bits(__lows2half2(value_hi, rest_hi)));
+          pf[0][2 * i + 1][0] = transpose8(bits(__highs2half2(value_lo, rest_lo)));
+          pf[0][2 * i + 1][1] = transpose8(bits(__highs2half2(value_hi, rest_hi)));
+        }
+      } else {
+        const __half2 w_lo = __floats2half2_rn(p_lo[0], p_lo[1]), x_lo = rest_of(p_lo[0], p_lo[1], w_lo);
+        const __half2 w_hi = __floats2half2_rn(p_hi[0], p_hi[1]), x_hi = rest_of(p_hi[0], p_hi[1], w_hi);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {  // two heads at a time
+          const __half2 d_lo = __hmul2(halves(dv_lo[b / 2]), to_range), d_hi = __hmul2(halves(dv_hi[b / 2]), to_range);
+          __half2 value_lo, rest_lo, value_hi, rest_hi;
+          product(w_lo, x_lo, b & 1 ? __high2half2(d_lo) : __low2half2(d_lo), value_lo, rest_lo);
+          product(w_hi, x_hi, b & 1 ? __high2half2(d_hi) : __low2half2(d_hi), value_hi, rest_hi);
+          pf[0][b][0] = transpose8(bits(value_lo));
+          pf[0][b][1] = transpose8(bits(value_hi));
+          pf[1][b][0] = transpose8(bits(rest_lo));
+          pf[1][b][1] = transpose8(bits(rest_hi));
         }
       }
       {
         __align__(8) uint32_t w[4][NB / 2];  // of tokens t, t + 4, t + 8, t + 12: columns 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        const unsigned char* v_codes = ring + at + Cfg::kRecord + t * (D / 2) + g * (2 * NB);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const unsigned char* src = vs + (4 * i + t) * (D / 2) + g * (2 * NB);
-          if constexpr (NB == 4) *reinterpret_cast<uint2*>(w[i]) = *reinterpret_cast<const uint2*>(src);
-          else w[i][0] = *reinterpret_cast<const uint32_t*>(src);
-        }
+        for (int i = 0; i < 4; ++i) load_words<NB / 2>(w[i], v_codes + 4 * i * (D / 2));
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           const unsigned pick = b & 1 ? 0x7632u : 0x5410u;
           const uint32_t x = __byte_perm(w[0][b / 2], w[1][b / 2], pick), y = __byte_perm(w[2][b / 2], w[3][b / 2], pick), x8 = x >> 8, y8 = y >> 8;
-          const uint32_t a00 = widen<true>(x), a01 = widen<false>(x), a02 = widen<true>(y), a03 = widen<false>(y);
-          const uint32_t a10 = widen<true>(x8), a11 = widen<false>(x8), a12 = widen<true>(y8), a13 = widen<false>(y8);
+          const uint32_t a00 = widen.get<true>(x), a01 = widen.get<false>(x), a02 = widen.get<true>(y), a03 = widen.get<false>(y);
+          const uint32_t a10 = widen.get<true>(x8), a11 = widen.get<false>(x8), a12 = widen.get<true>(y8), a13 = widen.get<false>(y8);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma(o[n][2 * b], a00, a01, a02, a03, pf[n][b][0], pf[n][b][1]);
-            mma(o[n][2 * b + 1], a10, a11, a12, a13, pf[n][b][0], pf[n][b][1]);
+          for (int p = 0; p < (PAIRS ? 1 : 2); ++p) {
+            mma(o[2 * b], a00, a01, a02, a03, pf[p][b][0], pf[p][b][1]);
+            mma(o[2 * b + 1], a10, a11, a12, a13, pf[p][b][0], pf[p][b][1]);
           }
         }
       }
       __syncwarp();
-      stage = (stage + 1) % kStages;
+      step(at);
     }
 
     // the unit's sums over the warps
-    const float back = top_scale / (float)(1 << kWeightBits);
+    const float back = 1.0f / __low2float(to_range);  // the weights' own 2^kWeightBits cancels against that of their sum
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int m = 0; m < MINE; ++m) {
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) weight[n] += __shfl_xor_sync(0xffffffffu, weight[n], off);
-      float* dst = sums + (warp * Cfg::kHeads + 4 * n + t) * Cfg::kPitch + g;
+      for (int off = 4; off < 32; off <<= 1) weight[m] += __shfl_xor_sync(0xffffffffu, weight[m], off);
+      const int at_head = warp * Cfg::kHeads + (PAIRS ? t : 2 * t + m);
+      float* dst = sums + at_head * Cfg::kPitch + g;
 #pragma unroll
       for (int i = 0; i < 2 * NB; ++i) {
-        dst[16 * i] = (o[n][i][0] + o[n][i][1]) * back;
-        dst[16 * i + 8] = (o[n][i][2] + o[n][i][3]) * back;
+        dst[16 * i] = (PAIRS ? o[i][0] + o[i][1] : o[i][m]) * back;
+        dst[16 * i + 8] = (PAIRS ? o[i][2] + o[i][3] : o[i][2 + m]) * back;
       }
       if (g == 0) {
-        refs[warp * Cfg::kHeads + 4 * n + t] = ref[n];
-        weights[warp * Cfg::kHeads + 4 * n + t] = weight[n];
+        refs[at_head] = ref[m];
+        weights[at_head] = weight[m];
       }
     }
     __syncthreads();
@@ -486,7 +575,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 16 / WARPS : 12 / WARPS)
         if (a.out) a.out[(size_t)run.lane * a.q_heads * D + k] = val;
         if (a.out_xh) a.out_xh[hand_off_cell(k >> 3, run.lane, a.out_xh_nv, a.q_heads * (D / 8)) + (k & 7)] = half_sat(val);
       } else {
-        float* dst = a.partial + ((size_t)(2 * blockIdx.x + (first_unit ? 0 : 1)) * a.heads + h) * (D + 2);
+        float* dst = a.partial + ((size_t)(2 * blockIdx.x + (first_unit ? 0 : 1)) * a.heads + h) * (D + kPartPad);
         dst[d] = acc;
         if (d == 0) { dst[D] = m; dst[D + 1] = l; }
       }
@@ -498,61 +587,85 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 16 / WARPS : 12 / WARPS)
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Adds up the parts of units that were cut, and clears the rows of lanes with nothing to attend over. Grid (units of a lane, lanes).
-__global__ void attention_q4_merge_kernel(Q4Args a, int D, int ctas) {
+// Adds up the parts of units that were cut, and clears the rows of lanes with nothing to attend over. Grid (units of a lane x heads of a
+// unit, lanes). Latency-bound: a CTA's eight warps take the parts in turn, a thread four columns of them; a reference is fetched
+// with its part. (One CTA per unit, a part after the other: 150 of 182 us for one lane in 37 parts.)
+constexpr int kMergeWarps = 8;
+template <int D>
+__global__ void __launch_bounds__(kMergeWarps * 32) attention_q4_merge_kernel(Q4Args a, int ctas) {
+  __shared__ __align__(16) float sums[kMergeWarps][D];
+  __shared__ float refs[kMergeWarps], weights[kMergeWarps];
+  constexpr int COLUMNS = D / 32;  // of a thread
   chain_release();
   chain_wait();
-  const int units = a.kv_heads * a.groups, unit = blockIdx.x, lane_id = blockIdx.y, G = a.q_heads / a.kv_heads;
-  const long long total = all_pages(a) * units;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int units = a.kv_heads * a.groups, unit = blockIdx.x / a.heads, h = blockIdx.x - unit * a.heads, lane_id = blockIdx.y, G = a.q_heads / a.kv_heads;
+  const int kv_head = unit / a.groups, head = kv_head * G + (unit - kv_head * a.groups) * a.heads + h;
+  if (head >= (kv_head + 1) * G) return;  // the last group may have fewer heads
+  long long all = 0, before = 0;
+  for (int i = lane; i < a.batch; i += 32) {
+    const int pages = span_of(a.lanes[i], a.op_window).pages;
+    all += places_of(pages);
+    if (i < lane_id) before += places_of(pages);
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, off);
+    before += __shfl_xor_sync(0xffffffffu, before, off);
+  }
   const int pages = span_of(a.lanes[lane_id], a.op_window).pages;
-  const int kv_head = unit / a.groups, head0 = kv_head * G + (unit - kv_head * a.groups) * a.heads;
-  const int live_heads = min(a.heads, (kv_head + 1) * G - head0);
-  auto store = [&](int h, int d, float val) {
-    const int k = (head0 + h) * D + d;
+  auto store = [&](int d, float val) {
+    const int k = head * D + d;
     if (a.out) a.out[(size_t)lane_id * a.q_heads * D + k] = val;
     if (a.out_xh) a.out_xh[hand_off_cell(k >> 3, lane_id, a.out_xh_nv, a.q_heads * (D / 8)) + (k & 7)] = half_sat(val);
   };
   if (pages == 0) {
-    for (int i = threadIdx.x; i < live_heads * D; i += blockDim.x) store(i / D, i % D, 0.0f);
+    if (threadIdx.x < D) store(threadIdx.x, 0.0f);
     return;
   }
-  long long before = 0;
-  for (int i = threadIdx.x & 31; i < lane_id; i += 32) before += span_of(a.lanes[i], a.op_window).pages;
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) before += __shfl_xor_sync(0xffffffffu, before, off);
-  const long long s = before * units + (long long)unit * pages, e = s + pages;
-  // the CTA that holds page x is the last whose run starts at or before it: total * c / ctas <= x
-  const int c0 = (int)(((s + 1) * ctas - 1) / total), c1 = (int)((e * ctas - 1) / total);
+  const long long total = all * units, s = before * units + (long long)unit * places_of(pages), e = s + places_of(pages);
+  // the CTA that holds place x is the last whose run starts at or before it: total * c / ctas <= x
+  const int c0 = (int)(((s + kUnitPages + 1) * ctas - 1) / total), c1 = (int)((e * ctas - 1) / total);
   if (c0 == c1) return;
-  // a run is empty where there are more CTAs than pages
-  auto empty = [&](int c) { return total * c / ctas == total * (c + 1) / ctas; };
-  auto part = [&](int c, int h) {
-    const int slot = total * c / ctas >= s ? 0 : 1;  // the run's first unit or its last
-    return a.partial + ((size_t)(2 * c + slot) * a.heads + h) * (D + 2);
-  };
-  for (int i = threadIdx.x; i < live_heads * D; i += blockDim.x) {
-    const int h = i / D, d = i - h * D;
-    float m = -INFINITY, acc = 0.0f, l = 0.0f;
-    for (int c = c0; c <= c1; ++c)
-      if (!empty(c)) m = fmaxf(m, part(c, h)[D]);
-    for (int c = c0; c <= c1; ++c) {
-      if (empty(c)) continue;
-      const float* p = part(c, h);
-      const float f = p[D] == -INFINITY ? 0.0f : exp2_flushed(p[D] - m);
-      acc += f * p[d];
-      l += f * p[D + 1];
-    }
-    store(h, d, l == 0.0f ? 0.0f : acc / l);
+  const int slot0 = total * c0 / ctas >= s ? 0 : 1;  // the run's first unit or its last; the others begin inside this unit
+  float m = -INFINITY, l = 0.0f, acc[COLUMNS] = {};
+  for (int c = c0 + warp; c <= c1; c += kMergeWarps) {
+    if (total < ctas && total * c / ctas == total * (c + 1) / ctas) continue;  // more CTAs than pages: an empty run
+    const float* part = a.partial + ((size_t)(2 * c + (c == c0 ? slot0 : 0)) * a.heads + h) * (D + kPartPad);
+    float x[COLUMNS];
+#pragma unroll
+    for (int j = 0; j < COLUMNS; ++j) x[j] = part[lane + 32 * j];
+    const float r = part[D], w = part[D + 1], to = fmaxf(m, r);
+    const float old = m == -INFINITY ? 0.0f : exp2_flushed(m - to), f = r == -INFINITY ? 0.0f : exp2_flushed(r - to);
+    m = to;
+    l = l * old + w * f;
+#pragma unroll
+    for (int j = 0; j < COLUMNS; ++j) acc[j] = acc[j] * old + x[j] * f;
   }
+#pragma unroll
+  for (int j = 0; j < COLUMNS; ++j) sums[warp][lane + 32 * j] = acc[j];
+  if (lane == 0) { refs[warp] = m; weights[warp] = l; }
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  float most = -INFINITY, sum = 0.0f, weight = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kMergeWarps; ++w) most = fmaxf(most, refs[w]);
+#pragma unroll
+  for (int w = 0; w < kMergeWarps; ++w) {
+    const float f = refs[w] == -INFINITY ? 0.0f : exp2_flushed(refs[w] - most);
+    sum += f * sums[w][threadIdx.x];
+    weight += f * weights[w];
+  }
+  store(threadIdx.x, weight == 0.0f ? 0.0f : sum / weight);
 }
 
 // Query heads of a KV head in groups of at most eight: with more the accumulators of a warp do not fit its registers.
 int head_groups(int q_heads, int kv_heads) { return (q_heads / kv_heads + 7) / 8; }
 
-template <int D, int NT, int WARPS>
+template <int D, bool PAIRS, int WARPS>
 cudaError_t launch_t(const Q4Args& a, unsigned ctas, cudaStream_t stream) {
-  auto kernel = attention_q4_kernel<D, NT, WARPS>;
-  constexpr size_t smem = Q4Cfg<D, NT, WARPS>::kSmem;
+  auto kernel = attention_q4_kernel<D, PAIRS, WARPS>;
+  constexpr size_t smem = Q4Cfg<D, PAIRS, WARPS>::kSmem;
   const cudaError_t e = opt_in_shared_memory(kernel, smem);
   if (e != cudaSuccess) return e;
   return launch_chained(kernel, dim3(ctas), dim3(WARPS * 32), smem, stream, a);
@@ -574,7 +687,7 @@ Q4Plan plan_attention_q4(int batch, int q_heads, int kv_heads, int head_dim, int
   p.direct = max_pages <= kDirectPages;
   // as many CTAs as are resident at once, but two pages for every warp where the tables are short
   p.ctas = p.direct ? units : std::min<int64_t>((int64_t)resident * sm_count, (units * max_pages + 2 * warps - 1) / (2 * warps));
-  p.scratch_bytes = p.direct ? 0 : (size_t)p.ctas * 2 * heads * (head_dim + 2) * sizeof(float);
+  p.scratch_bytes = p.direct ? 0 : (size_t)p.ctas * 2 * heads * (head_dim + kPartPad) * sizeof(float);
   return p;
 }
 
@@ -602,12 +715,13 @@ cudaError_t launch_attention_q4(const PoolView& pool, const float* q, const Lane
   a.op_window = op_window;
   const unsigned ctas = (unsigned)plan.ctas;
   cudaError_t e;
-  if (a.heads <= 4) e = pool.head_dim == 128 ? launch_t<128, 1, 8>(a, ctas, stream) : launch_t<64, 1, 8>(a, ctas, stream);
-  else e = pool.head_dim == 128 ? launch_t<128, 2, 4>(a, ctas, stream) : launch_t<64, 2, 4>(a, ctas, stream);
+  if (a.heads <= 4) e = pool.head_dim == 128 ? launch_t<128, true, 8>(a, ctas, stream) : launch_t<64, true, 8>(a, ctas, stream);
+  else e = pool.head_dim == 128 ? launch_t<128, false, 4>(a, ctas, stream) : launch_t<64, false, 4>(a, ctas, stream);
   if (e != cudaSuccess) return e;
   if (launches) ++*launches;
   if (plan.direct) return cudaSuccess;
-  e = launch_chained(attention_q4_merge_kernel, dim3((unsigned)(a.kv_heads * a.groups), (unsigned)batch), dim3(128), 0, stream, a, pool.head_dim, (int)plan.ctas);
+  const dim3 grid((unsigned)(a.kv_heads * a.groups * a.heads), (unsigned)batch);
+  e = launch_chained(pool.head_dim == 128 ? attention_q4_merge_kernel<128> : attention_q4_merge_kernel<64>, grid, dim3(kMergeWarps * 32), 0, stream, a, (int)plan.ctas);
   if (e == cudaSuccess && launches) ++*launches;
   return e;
 }
