@@ -16,10 +16,12 @@
 //
 // What bounds it is the issue rate, not HBM: some 400 instructions per page and warp, 152 of them widening codes.
 //
-// Work. The pages of all (lane, KV head) units in a row are cut into as many equal runs as there are CTAs, whatever the lengths of the
-// lanes: no CTA waits for the longest. Warps take a run's pages in turn through a ring of cp.async copies that runs on across the
-// units. A unit within one run is finished there; the parts of one that is cut go to scratch (two per CTA at most) and a second kernel
-// adds them up. Short tables (kDirectPages) take one CTA per unit and no second kernel.
+// Work. The pages of all (lane, KV head) units in a row are cut into as many equal runs as there are warps, whatever the lengths of the
+// lanes: nobody waits for the longest. A warp takes its run page by page through a ring of cp.async copies that runs on across units, and
+// writes the units that lie inside it. What neighbouring warps of a CTA have of one unit is added up in shared memory at the end;
+// the parts of a unit that several CTAs share go to scratch (two per CTA at most) and a second kernel adds them up. Short tables
+// (kDirectPages) take one CTA per unit and no second kernel. (Runs of whole CTAs, whose warps took pages in turn and met after each
+// unit: 67 us against XX for 64 lanes of 128 to 4096 tokens.)
 //
 // Scores are compared with a reference that is raised, with everything accumulated, only when one exceeds it by 2^kSlack: a few times per
 // run instead of once per page.
@@ -39,11 +41,20 @@ namespace {
 constexpr int kPage = 16;
 constexpr int kStages = 3;
 constexpr int kDirectPages = 16;
-constexpr int kUnitPages = 12;  // what a unit costs beyond its pages, in pages
+constexpr int kUnitPages = 6;  // what a unit costs beyond its pages, in pages
 constexpr int kPartPad = 4;  // of a head's part: reference, sum of weights, two unused
 constexpr float kSlack = 6.0f;
 constexpr float kWeightBits = 8.0f;  // weights are scaled by 2^8: at most 2^14 with the slack
 constexpr float kSmallestScale = 5.9604645e-8f;  // 2^-24, the smallest f16
+
+// What a CTA has of units that other CTAs have parts of: the end of one that began before it (part 0), the beginning of one that goes on
+// behind it (part 1).
+struct Ends {
+  int open, open_ends;  // there is a part 0; the unit ends in it
+  int tail;             // there is a part 1, of:
+  int row, head0, heads;
+  int unused[2];
+};
 
 struct Q4Args {
   const uint8_t* k;
@@ -55,6 +66,7 @@ struct Q4Args {
   __half* out_xh;  // optional: in the hand-off layout
   int out_xh_nv;
   float* partial;  // [CTAs][2][heads of a unit][D + kPartPad]: O, then reference and sum of the weights
+  struct Ends* ends;  // [CTAs]
   int batch, q_heads, kv_heads;
   int groups, heads;  // query-head groups per KV head, heads of a group (the last may have fewer)
   int direct;
@@ -165,6 +177,12 @@ __device__ __forceinline__ float to_f16_range(float x) {
   return __uint_as_float((unsigned)min(max(127 + 13 - (e - 127), 1), 254) << 23);
 }
 
+// Column k of a lane's output row.
+__device__ __forceinline__ void store_out(const Q4Args& a, int D, int row, int k, float val) {
+  if (a.out) a.out[(size_t)row * a.q_heads * D + k] = val;
+  if (a.out_xh) a.out_xh[hand_off_cell(k >> 3, row, a.out_xh_nv, a.q_heads * (D / 8)) + (k & 7)] = half_sat(val);
+}
+
 // What V scales are multiplied by, of which no |dv| exceeds the power of two `top`: 1 / top, as far as f16 holds it.
 __device__ __forceinline__ __half2 scale_to_range(float top) { return __float2half2_rn(fminf(1.0f / top, 32768.0f)); }
 
@@ -177,7 +195,7 @@ struct Q4Cfg {
   static constexpr int kHeads = PAIRS ? 4 : 8;
   static constexpr int kPitch = D + 8;                          // of a head's partial sums: no bank conflicts
   static constexpr int kRing = WARPS * kStages * kStage;
-  static constexpr size_t kSmem = kRing + (size_t)WARPS * kHeads * (kPitch + 2) * sizeof(float);
+  static constexpr size_t kSmem = kRing + (size_t)2 * WARPS * kHeads * (kPitch + 2) * sizeof(float);
 };
 
 // N words (1, 2 or 4) from shared memory, aligned to their size.
@@ -188,7 +206,13 @@ __device__ __forceinline__ void load_words(uint32_t* dst, const unsigned char* s
   else dst[0] = *reinterpret_cast<const uint32_t*>(src);
 }
 
-// A run of work, page by page for one warp: the unit it is in and its next page there.
+// What a warp has of a unit that lies not wholly in its run.
+struct Record {
+  int valid, ends;     // ends: the unit's last page is in it
+  int row, head0, heads;
+};
+
+// A warp's run of work: the unit it is in and its pages there.
 struct Cursor {
   long long at, stop;  // the places where the unit, or the run, ends
   int lane, unit;      // unit: KV head * groups + group
@@ -234,39 +258,56 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
     }
     return false;
   };
+  if (!a.direct) {  // lanes with nothing to attend over
+    for (int l = blockIdx.x; l < a.batch; l += gridDim.x)
+      if (span_of(a.lanes[l], a.op_window).pages == 0)
+        for (int i = threadIdx.x; i < a.q_heads * D; i += WARPS * 32) store_out(a, D, l, i, 0.0f);
+  }
+  __shared__ Record records[2 * WARPS];  // of each warp the unit that began before its run, the unit that goes on behind it
+  if (lane < 2) records[2 * warp + lane].valid = 0;
+  bool works = true;
   if (a.direct) {
     run.lane = blockIdx.x / units;
     run.unit = blockIdx.x - run.lane * units;
-    run.at = 0;
     enter(run);
-    run.stop = places_of(run.span.pages);
-    clip(run, 0);
+    if (run.span.pages == 0) {  // nothing to attend over
+      const int kv_head = run.unit / a.groups, head0 = kv_head * G + (run.unit - kv_head * a.groups) * a.heads;
+      for (int i = threadIdx.x; i < min(a.heads, (kv_head + 1) * G - head0) * D; i += WARPS * 32) store_out(a, D, run.lane, head0 * D + i, 0.0f);
+      return;
+    }
+    const int from = run.span.pages * warp / WARPS;
+    run.at = kUnitPages + from;
+    run.stop = kUnitPages + run.span.pages * (warp + 1) / WARPS;
+    works = run.at < run.stop;
+    clip(run, kUnitPages + from);
   } else {
     const long long total = all_places(a) * units;
-    const long long begin = total * blockIdx.x / gridDim.x;
-    run.stop = total * (blockIdx.x + 1) / gridDim.x;
-    if (begin >= run.stop) return;
-    long long before;
-    lane_at(a, begin, units, &run.lane, &before);
-    enter(run);
-    run.at = begin;
-    const long long inside = begin - before;
-    const int places = places_of(run.span.pages);
-    run.unit = (int)(inside / places);
-    clip(run, (int)(inside - (long long)run.unit * places));
-    if (run.page0 == run.page1 && !advance(run)) return;
+    const int runs = (int)gridDim.x * WARPS, mine = (int)blockIdx.x * WARPS + warp;
+    const long long begin = total * mine / runs;
+    run.stop = total * (mine + 1) / runs;
+    works = begin < run.stop;
+    if (works) {
+      long long before;
+      lane_at(a, begin, units, &run.lane, &before);
+      enter(run);
+      run.at = begin;
+      const long long inside = begin - before;
+      const int places = places_of(run.span.pages);
+      run.unit = (int)(inside / places);
+      clip(run, (int)(inside - (long long)run.unit * places));
+      works = run.page0 < run.page1 || advance(run);
+    }
   }
-  const bool idle = run.page0 == run.page1;  // direct: a lane with nothing to attend over
 
   // the ring: this warp's pages, from `ahead`, the cursor that copies are issued from; the number of the page that comes next is
   // looked up one copy ahead
   unsigned char* ring = smem + warp * (kStages * Cfg::kStage);
   const unsigned ring_at = (unsigned)__cvta_generic_to_shared(ring) + lane * 16;
   Cursor ahead = run;
-  int ahead_page = run.page0 + warp;
+  int ahead_page = run.page0;
   unsigned ahead_number = 0;
   const uint8_t *ahead_k, *ahead_v;  // page 0 of the unit's KV head, this lane's 16 bytes
-  bool more = !idle;
+  bool more = works;
   const unsigned page_stride = (unsigned)(a.kv_heads * Cfg::kRecord);
   auto aim = [&] {
     const size_t from = (size_t)(ahead.unit / a.groups) * Cfg::kRecord + lane * 16;
@@ -276,13 +317,15 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
   auto look_up = [&] {
     while (more && ahead_page >= ahead.page1) {
       more = advance(ahead);
-      ahead_page = ahead.page0 + warp;
+      ahead_page = ahead.page0;
       aim();
     }
     if (more) ahead_number = (unsigned)a.tables[ahead.table + ahead_page];
   };
-  aim();
-  look_up();
+  if (works) {
+    aim();
+    look_up();
+  }
   auto issue = [&](unsigned offset) {
     if (more) {
       const uint8_t *k = ahead_k + (unsigned long long)ahead_number * page_stride, *v = ahead_v + (unsigned long long)ahead_number * page_stride;
@@ -293,7 +336,7 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
           copy16(dst + c, k + c);
           copy16(dst + Cfg::kRecord + c, v + c);
         }
-      ahead_page += WARPS;
+      ++ahead_page;
       look_up();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -306,14 +349,13 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
     step(fill);
   }
 
-  float* sums = reinterpret_cast<float*>(smem + Cfg::kRing);  // [warp][head][pitch], then references and weights [warp][head]
-  float* refs = sums + WARPS * Cfg::kHeads * Cfg::kPitch;
-  float* weights = refs + WARPS * Cfg::kHeads;
+  float* sums = reinterpret_cast<float*>(smem + Cfg::kRing);  // [record][head][pitch], then references and weights [record][head]
+  float* refs = sums + 2 * WARPS * Cfg::kHeads * Cfg::kPitch;
+  float* weights = refs + 2 * WARPS * Cfg::kHeads;
   const int row_lo = (g >> 1) + 4 * (g & 1);  // tokens of this thread's scores, row_lo and row_lo + 8: row r of a tile is token r/2 + 4 (r%2)
   const Widen widen;
   const bool wide_q = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;
-  bool first_unit = true;
-  while (true) {
+  while (works) {
     const int kv_head = run.unit / a.groups, head0 = kv_head * G + (run.unit - kv_head * a.groups) * a.heads;
     const int live_heads = min(a.heads, (kv_head + 1) * G - head0);
     // queries: column g is the value (g even) or the rest (g odd) of head g / 2, or value and rest, one after the other, of head g
@@ -369,7 +411,7 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
     __half2 top_half = __float2half2_rn(top_scale), to_range = scale_to_range(top_scale);
     const int inner0 = (run.span.begin + kPage - 1) / kPage, inner1 = run.span.end / kPage;  // pages without a masked token
 
-    for (int page = run.page0 + warp; page < run.page1; page += WARPS) {
+    for (int page = run.page0; page < run.page1; ++page) {
       issue(fill);
       step(fill);
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
@@ -538,58 +580,89 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
       step(at);
     }
 
-    // the unit's sums over the warps
+    // a whole unit is written, a part of one kept for the end
     const float back = 1.0f / __low2float(to_range);  // the weights' own 2^kWeightBits cancels against that of their sum
+    const bool begins = run.page0 == run.span.first, ends = run.page1 == run.span.first + run.span.pages;
+    const int record = 2 * warp + (begins ? 1 : 0);
+    if (lane == 0 && !(begins && ends)) records[record] = Record{1, ends, run.lane, head0, live_heads};
 #pragma unroll
     for (int m = 0; m < MINE; ++m) {
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) weight[m] += __shfl_xor_sync(0xffffffffu, weight[m], off);
-      const int at_head = warp * Cfg::kHeads + (PAIRS ? t : 2 * t + m);
-      float* dst = sums + at_head * Cfg::kPitch + g;
+      const int h = PAIRS ? t : 2 * t + m;
+      const float f = begins && ends ? (weight[m] == 0.0f ? 0.0f : back / weight[m]) : back;
+      float* dst = sums + (record * Cfg::kHeads + h) * Cfg::kPitch + g;
 #pragma unroll
-      for (int i = 0; i < 2 * NB; ++i) {
-        dst[16 * i] = (PAIRS ? o[i][0] + o[i][1] : o[i][m]) * back;
-        dst[16 * i + 8] = (PAIRS ? o[i][2] + o[i][3] : o[i][2 + m]) * back;
+      for (int i = 0; i < 4 * NB; ++i) {  // columns 8 i + g
+        const float val = (PAIRS ? o[i / 2][2 * (i & 1)] + o[i / 2][2 * (i & 1) + 1] : o[i / 2][2 * (i & 1) + m]) * f;
+        if (!(begins && ends)) dst[8 * i] = val;
+        else if (h < live_heads) store_out(a, D, run.lane, (head0 + h) * D + 8 * i + g, val);
       }
       if (g == 0) {
-        refs[at_head] = ref[m];
-        weights[at_head] = weight[m];
+        refs[record * Cfg::kHeads + h] = ref[m];
+        weights[record * Cfg::kHeads + h] = weight[m];
       }
     }
-    __syncthreads();
-    const bool whole = run.page0 == run.span.first && run.page1 == run.span.first + run.span.pages;
-    for (int i = threadIdx.x; i < live_heads * D; i += WARPS * 32) {
+    works = advance(run);
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+
+  // Units that more than one warp has: a record of a unit that begins in this CTA, or the first of one that began before it, and the records
+  // behind it up to the unit's end.
+  const bool mine = lane < 2 * WARPS && records[lane % (2 * WARPS)].valid;
+  unsigned left = __ballot_sync(0xffffffffu, mine);
+  const unsigned last = __ballot_sync(0xffffffffu, mine && records[lane % (2 * WARPS)].ends);
+  Ends mine_of = {};
+  while (left) {
+    const int k = __ffs(left) - 1, end = __ffs(left & last);  // 0: the unit goes on behind this CTA
+    const bool open = (k & 1) == 0;                           // it began in an earlier one
+    const unsigned members = end ? left & (0xffffffffu >> (32 - end)) : left;
+    left &= ~members;
+    const Record first = records[k];
+    if (open) {
+      mine_of.open = 1;
+      mine_of.open_ends = end != 0;
+    } else if (!end) {
+      mine_of.tail = 1;
+      mine_of.row = first.row;
+      mine_of.head0 = first.head0;
+      mine_of.heads = first.heads;
+    }
+    for (int i = threadIdx.x; i < first.heads * D; i += WARPS * 32) {
       const int h = i / D, d = i - h * D;
-      float m = -INFINITY, acc = 0.0f, l = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) m = fmaxf(m, refs[w * Cfg::kHeads + h]);
+      float ref[WARPS], m = -INFINITY, acc = 0.0f, l = 0.0f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float r = refs[w * Cfg::kHeads + h], f = r == -INFINITY ? 0.0f : exp2_flushed(r - m);
-        acc += f * sums[(w * Cfg::kHeads + h) * Cfg::kPitch + d];
-        l += f * weights[w * Cfg::kHeads + h];
+        const int r = w == k / 2 ? k : 2 * w;
+        ref[w] = members >> r & 1 ? refs[r * Cfg::kHeads + h] : -INFINITY;
+        m = fmaxf(m, ref[w]);
       }
-      if (whole || idle) {
-        const float val = l == 0.0f ? 0.0f : acc / l;
-        const int k = (head0 + h) * D + d;
-        if (a.out) a.out[(size_t)run.lane * a.q_heads * D + k] = val;
-        if (a.out_xh) a.out_xh[hand_off_cell(k >> 3, run.lane, a.out_xh_nv, a.q_heads * (D / 8)) + (k & 7)] = half_sat(val);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const int r = w == k / 2 ? k : 2 * w;
+        const float f = ref[w] == -INFINITY ? 0.0f : exp2_flushed(ref[w] - m);
+        if (members >> r & 1) {
+          acc = fmaf(f, sums[(r * Cfg::kHeads + h) * Cfg::kPitch + d], acc);
+          l = fmaf(f, weights[r * Cfg::kHeads + h], l);
+        }
+      }
+      if (!open && end) {
+        store_out(a, D, first.row, (first.head0 + h) * D + d, l == 0.0f ? 0.0f : acc / l);
       } else {
-        float* dst = a.partial + ((size_t)(2 * blockIdx.x + (first_unit ? 0 : 1)) * a.heads + h) * (D + kPartPad);
+        float* dst = a.partial + ((size_t)(2 * blockIdx.x + (open ? 0 : 1)) * a.heads + h) * (D + kPartPad);
         dst[d] = acc;
         if (d == 0) { dst[D] = m; dst[D + 1] = l; }
       }
     }
-    first_unit = false;
-    if (idle || !advance(run)) break;
-    __syncthreads();  // the sums have been read
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (!a.direct && threadIdx.x == 0) a.ends[blockIdx.x] = mine_of;
 }
 
-// Adds up the parts of units that were cut, and clears the rows of lanes with nothing to attend over. Grid (units of a lane x heads of a
-// unit, lanes). Latency-bound: a CTA's eight warps take the parts in turn, a thread four columns of them; a reference is fetched
-// with its part. (One CTA per unit, a part after the other: 150 of 182 us for one lane in 37 parts.)
+// Adds up the parts of units that were cut: grid (heads of a unit, CTAs of the attention kernel), a CTA for the unit that goes on behind
+// its namesake, if there is one. Latency-bound: eight warps take the parts in turn, a thread D / 32 columns of them; a reference is
+// fetched with its part. (One CTA per unit, a part after the other: 150 of 182 us for one lane in 37 parts; a CTA for every unit and
+// head, which worked out by 64-bit divisions whether its unit was cut: 14 us for 64 lanes.)
 constexpr int kMergeWarps = 8;
 template <int D>
 __global__ void __launch_bounds__(kMergeWarps * 32) attention_q4_merge_kernel(Q4Args a, int ctas) {
@@ -598,40 +671,22 @@ __global__ void __launch_bounds__(kMergeWarps * 32) attention_q4_merge_kernel(Q4
   constexpr int COLUMNS = D / 32;  // of a thread
   chain_release();
   chain_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int units = a.kv_heads * a.groups, unit = blockIdx.x / a.heads, h = blockIdx.x - unit * a.heads, lane_id = blockIdx.y, G = a.q_heads / a.kv_heads;
-  const int kv_head = unit / a.groups, head = kv_head * G + (unit - kv_head * a.groups) * a.heads + h;
-  if (head >= (kv_head + 1) * G) return;  // the last group may have fewer heads
-  long long all = 0, before = 0;
-  for (int i = lane; i < a.batch; i += 32) {
-    const int pages = span_of(a.lanes[i], a.op_window).pages;
-    all += places_of(pages);
-    if (i < lane_id) before += places_of(pages);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.x, c0 = blockIdx.y;
+  const Ends own = a.ends[c0];
+  if (!own.tail || h >= own.heads) return;
+  int c1 = c0;  // the CTA in which the unit ends: the first behind c0 whose open unit does
+  for (int from = c0 + 1; from < ctas; from += 32) {
+    const int c = from + lane;
+    const unsigned found = __ballot_sync(0xffffffffu, c < ctas && a.ends[c].open_ends);
+    if (found) {
+      c1 = from + __ffs(found) - 1;
+      break;
+    }
   }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, off);
-    before += __shfl_xor_sync(0xffffffffu, before, off);
-  }
-  const int pages = span_of(a.lanes[lane_id], a.op_window).pages;
-  auto store = [&](int d, float val) {
-    const int k = head * D + d;
-    if (a.out) a.out[(size_t)lane_id * a.q_heads * D + k] = val;
-    if (a.out_xh) a.out_xh[hand_off_cell(k >> 3, lane_id, a.out_xh_nv, a.q_heads * (D / 8)) + (k & 7)] = half_sat(val);
-  };
-  if (pages == 0) {
-    if (threadIdx.x < D) store(threadIdx.x, 0.0f);
-    return;
-  }
-  const long long total = all * units, s = before * units + (long long)unit * places_of(pages), e = s + places_of(pages);
-  // the CTA that holds place x is the last whose run starts at or before it: total * c / ctas <= x
-  const int c0 = (int)(((s + kUnitPages + 1) * ctas - 1) / total), c1 = (int)((e * ctas - 1) / total);
-  if (c0 == c1) return;
-  const int slot0 = total * c0 / ctas >= s ? 0 : 1;  // the run's first unit or its last; the others begin inside this unit
   float m = -INFINITY, l = 0.0f, acc[COLUMNS] = {};
   for (int c = c0 + warp; c <= c1; c += kMergeWarps) {
-    if (total < ctas && total * c / ctas == total * (c + 1) / ctas) continue;  // more CTAs than pages: an empty run
-    const float* part = a.partial + ((size_t)(2 * c + (c == c0 ? slot0 : 0)) * a.heads + h) * (D + kPartPad);
+    if (c > c0 && !a.ends[c].open) continue;  // more CTAs than places: it has none
+    const float* part = a.partial + ((size_t)(2 * c + (c == c0 ? 1 : 0)) * a.heads + h) * (D + kPartPad);
     float x[COLUMNS];
 #pragma unroll
     for (int j = 0; j < COLUMNS; ++j) x[j] = part[lane + 32 * j];
@@ -656,7 +711,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) attention_q4_merge_kernel(Q4
     sum += f * sums[w][threadIdx.x];
     weight += f * weights[w];
   }
-  store(threadIdx.x, weight == 0.0f ? 0.0f : sum / weight);
+  store_out(a, D, own.row, (own.head0 + h) * D + threadIdx.x, weight == 0.0f ? 0.0f : sum / weight);
 }
 
 // Query heads of a KV head in groups of at most eight: with more the accumulators of a warp do not fit its registers.
@@ -687,7 +742,7 @@ Q4Plan plan_attention_q4(int batch, int q_heads, int kv_heads, int head_dim, int
   p.direct = max_pages <= kDirectPages;
   // as many CTAs as are resident at once, but two pages for every warp where the tables are short
   p.ctas = p.direct ? units : std::min<int64_t>((int64_t)resident * sm_count, (units * max_pages + 2 * warps - 1) / (2 * warps));
-  p.scratch_bytes = p.direct ? 0 : (size_t)p.ctas * 2 * heads * (head_dim + kPartPad) * sizeof(float);
+  p.scratch_bytes = p.direct ? 0 : (size_t)p.ctas * (2 * heads * (head_dim + kPartPad) * sizeof(float) + sizeof(Ends));
   return p;
 }
 
@@ -704,12 +759,13 @@ cudaError_t launch_attention_q4(const PoolView& pool, const float* q, const Lane
   a.out = out;
   a.out_xh = out_xh;
   a.out_xh_nv = xh_nv;
-  a.partial = scratch;
   a.batch = batch;
   a.q_heads = q_heads;
   a.kv_heads = pool.kv_heads;
   a.groups = head_groups(q_heads, pool.kv_heads);
   a.heads = (q_heads / pool.kv_heads + a.groups - 1) / a.groups;
+  a.partial = scratch;
+  a.ends = reinterpret_cast<Ends*>(scratch + (size_t)plan.ctas * 2 * a.heads * (pool.head_dim + kPartPad));
   a.direct = plan.direct;
   a.scale_log2 = (float)(scale * 1.4426950408889634);
   a.op_window = op_window;
@@ -720,8 +776,8 @@ cudaError_t launch_attention_q4(const PoolView& pool, const float* q, const Lane
   if (e != cudaSuccess) return e;
   if (launches) ++*launches;
   if (plan.direct) return cudaSuccess;
-  const dim3 grid((unsigned)(a.kv_heads * a.groups * a.heads), (unsigned)batch);
-  e = launch_chained(pool.head_dim == 128 ? attention_q4_merge_kernel<128> : attention_q4_merge_kernel<64>, grid, dim3(kMergeWarps * 32), 0, stream, a, (int)plan.ctas);
+  e = launch_chained(pool.head_dim == 128 ? attention_q4_merge_kernel<128> : attention_q4_merge_kernel<64>, dim3((unsigned)a.heads, ctas), dim3(kMergeWarps * 32), 0,
+                     stream, a, (int)plan.ctas);
   if (e == cudaSuccess && launches) ++*launches;
   return e;
 }
