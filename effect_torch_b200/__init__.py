@@ -552,7 +552,9 @@ class Executable:
 
     def __init__(self, rt: Runtime, *, layers, d_model, q_heads, kv_heads, head_dim, ffn, vocab, rms_eps=1e-5, rope_theta=10000.0,
                  rope_layout=HALF_SPLIT, window=None, batch=1, max_tokens=256, block_size=16, kv_dtype=KV_F32, exact=False,
-                 max_advance=1, vocab_global=None, head_first_row=0):
+                 max_advance=1, vocab_global=None, head_first_row=0, rope=None, rope_divisors=None):
+        """rope: a rope_config() that stands for rope_theta and rope_layout (scaled positions, part of a head), rope_divisors: one
+        frequency divisor per pair."""
         self.rt = rt
         self.cfg = DecoderConfig(layers, d_model, q_heads, kv_heads, head_dim, ffn, vocab, rms_eps, rope_theta, rope_layout,
                                  NO_WINDOW if window is None else window, batch, max_tokens, block_size, kv_dtype, int(exact))
@@ -560,6 +562,10 @@ class Executable:
         _check(rt.L.etc_decoder_create(rt.h, C.byref(self.cfg), C.byref(h)))
         self.h = h
         _check(rt.L.etc_decoder_set_max_advance(self.h, max_advance))
+        if rope is not None or rope_divisors is not None:
+            rope = rope_config(head_dim, theta=rope_theta, layout=rope_layout) if rope is None else rope
+            d = _divisors(rope, rope_divisors)
+            _check(rt.L.etc_decoder_set_rope(self.h, C.byref(rope), _ptr(d)))
         if vocab_global is not None:  # vocabulary-parallel head: `vocab` rows of it from `head_first_row` on
             _check(rt.L.etc_decoder_set_head_shard(self.h, vocab_global, head_first_row))
         self.vocab, self.batch = vocab, batch
@@ -643,6 +649,22 @@ class Executable:
         _check(self.rt.L.etc_decoder_execute_sampled(self.h, pool.h, self._seq_array(seqs), active, _ptr(tokens), advance, _ptr(out),
                                                      C.cast(C.byref(flag), C.c_void_p)))
         return out
+
+    def score(self, pool, seqs, tokens, targets, top: int = 0, cancelled: bool = False):
+        """Feeds tokens [active, advance] and returns, for each, the log probability of the token that follows it (targets, same shape), the
+        entropy and the `top` most likely tokens with their log probabilities: (logprobs, entropy, top_tokens, top_logprobs)."""
+        tokens = np.ascontiguousarray(tokens, dtype=np.uint32)
+        targets = np.ascontiguousarray(targets, dtype=np.uint32)
+        active, advance = tokens.shape
+        if targets.shape != tokens.shape:
+            raise BackendError(9, f"score: targets of shape {targets.shape} for tokens of shape {tokens.shape}")
+        rows = max(top, 0)
+        logprobs, entropy = np.empty((active, advance), np.float32), np.empty((active, advance), np.float32)
+        top_tokens, top_logprobs = np.empty((active, advance, rows), np.uint32), np.empty((active, advance, rows), np.float32)
+        flag = C.c_int(int(cancelled))
+        _check(self.rt.L.etc_decoder_score(self.h, pool.h, self._seq_array(seqs), active, _ptr(tokens), advance, _ptr(targets), _ptr(logprobs), _ptr(entropy),
+                                           top, _ptr(top_tokens), _ptr(top_logprobs), C.cast(C.byref(flag), C.c_void_p)))
+        return logprobs, entropy, top_tokens, top_logprobs
 
     def generate_greedy(self, pool, seqs, first_tokens, steps: int):
         first = np.ascontiguousarray(first_tokens, dtype=np.uint32).reshape(-1)

@@ -281,7 +281,7 @@ static size_t exact_step_smem(int head_dim, int max_ctx) {
 }
 
 __global__ void __launch_bounds__(128) attention_exact_step_kernel(PoolView pool, const float* qkv, const LaneInfo* lanes, const int* tables,
-                                                                   const double* inv_freq, int layout, int q_heads, double scale,
+                                                                   RopeView rope, int q_heads, double scale,
                                                                    long long op_window, float* out, int slots) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ double red[4];
@@ -317,11 +317,7 @@ __global__ void __launch_bounds__(128) attention_exact_step_kernel(PoolView pool
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(vd), "l"(reinterpret_cast<const float*>(pool.v) + src) : "memory");
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
-  for (int j = threadIdx.x; j < half; j += blockDim.x) {
-    double s, c;
-    sincos((double)info.cursor * inv_freq[j], &s, &c);
-    angle[j] = make_double2(s, c);
-  }
+  for (int j = threadIdx.x; j < half; j += blockDim.x) angle[j] = rope.angle(info.cursor, j);
   __syncthreads();  // the angles
   chain_wait();
   const size_t fresh = row_of(info.cursor) * D;
@@ -329,10 +325,10 @@ __global__ void __launch_bounds__(128) attention_exact_step_kernel(PoolView pool
   const float* row = qkv + (size_t)lane_id * (q_heads + 2 * pool.kv_heads) * D;
   for (int i = threadIdx.x; i < 3 * half; i += blockDim.x) {
     const int what = i / half, j = i - what * half;  // 0: query, 1: key, 2: value
-    const int i0 = layout == 0 ? j : 2 * j, i1 = layout == 0 ? half + j : 2 * j + 1;
+    const int i0 = rope.first(j), i1 = rope.second(j);
     const float* src = row + (size_t)(what == 0 ? head : q_heads + (what - 1) * pool.kv_heads + kv_head) * D;
     float r0 = src[i0], r1 = src[i1];
-    if (what < 2) {
+    if (what < 2 && j < rope.rotary_half) {
       const double first = (double)r0, second = (double)r1, s = angle[j].x, c = angle[j].y;
       r0 = (float)__dsub_rn(__dmul_rn(first, c), __dmul_rn(second, s));
       r1 = (float)__dadd_rn(__dmul_rn(second, c), __dmul_rn(first, s));
@@ -402,13 +398,13 @@ bool attention_exact_step_supported(const PoolView& pool, int batch, int q_heads
   return pool.head_dim >= 128 ? at_once > 2 || ctas <= 12ll * sm_count : at_once > 1 || ctas <= 16ll * sm_count;
 }
 
-cudaError_t launch_attention_exact_step(const PoolView& pool, const float* qkv, const LaneInfo* lanes, const int* tables, const double* inv_freq, int layout,
+cudaError_t launch_attention_exact_step(const PoolView& pool, const float* qkv, const LaneInfo* lanes, const int* tables, const RopeView& rope,
                                         int batch, int q_heads, double scale, long long op_window, float* out, int max_ctx, cudaStream_t stream) {
   if (batch == 0) return cudaSuccess;
   const cudaError_t attr = opt_in_shared_memory(attention_exact_step_kernel, kExactStepSmem);
   if (attr != cudaSuccess) return attr;
   return launch_chained(attention_exact_step_kernel, dim3((unsigned)q_heads, (unsigned)batch), dim3(128), exact_step_smem(pool.head_dim, max_ctx), stream, pool,
-                        qkv, lanes, tables, inv_freq, layout, q_heads, scale, op_window, out, exact_step_slots(max_ctx));
+                        qkv, lanes, tables, rope, q_heads, scale, op_window, out, exact_step_slots(max_ctx));
 }
 
 // --------------------------------------------------------------------------------------------
@@ -499,8 +495,7 @@ struct AttnArgs {
 struct FusedAttnArgs : AttnArgs {
   const float* qkv;
   DeferredSum sum;
-  const double* inv_freq;
-  int rope_layout;
+  RopeView rope;
   void *slab[2];           // K and V again, to store the new rows
   float *slab_scale[2];
 };
@@ -661,14 +656,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attention_mma_kernel(std::con
     __shared__ float fresh[2][D];    // the new K row, the new V row
     const int j = threadIdx.x % HALF, h0 = threadIdx.x / HALF;
     const bool works = p0 < p1, appends = works && new_page < p1;
-    if (works && h0 == 0) {
-      double sine, cosine;
-      sincos((double)info.cursor * a.inv_freq[j], &sine, &cosine);
-      angle[j] = make_double2(sine, cosine);
-    }
+    if (works && h0 == 0) angle[j] = a.rope.angle(info.cursor, j);
     chain_wait();
     if (works) {  // the same for the whole CTA
-      const int i0 = a.rope_layout == 0 ? j : 2 * j, i1 = a.rope_layout == 0 ? HALF + j : 2 * j + 1;
+      const int i0 = a.rope.first(j), i1 = a.rope.second(j);
       const int heads = a.q_heads + 2 * a.kv_heads, mine = appends ? G + 2 : G;
       auto head_of = [&](int h) { return h < G ? kv_head * G + h : a.q_heads + (h - G) * a.kv_heads + kv_head; };
       const size_t split_stride = (size_t)a.sum.vpad * a.sum.rows_padded;
@@ -705,7 +696,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attention_mma_kernel(std::con
           const int h = hb + u * STEP;
           if (h >= mine) break;
           float r0 = x0[u], r1 = x1[u];
-          if (h <= G) {  // not the value row
+          if (h <= G && j < a.rope.rotary_half) {  // not the value row
             const double first = (double)r0, second = (double)r1;
             r0 = (float)__dsub_rn(__dmul_rn(first, cosine), __dmul_rn(second, sine));
             r1 = (float)__dadd_rn(__dmul_rn(second, cosine), __dmul_rn(first, sine));
@@ -1003,13 +994,14 @@ constexpr int kChunkRows = 64;       // MMA rows per CTA
 constexpr int kChunkTokens = 64;     // cached positions per step
 constexpr int kChunkPages = kChunkTokens / kPageTokens;
 
-template <int D, bool U8>
+enum ChunkTier : int { kChunkHalves = 0, kChunkBytes = 1, kChunkQ4 = 2 };  // f16 or bf16; the int8 tier; the 4-bit tier
+template <int D, int TIER>
 struct ChunkCfg {
   static constexpr int kSide = kChunkTokens * D * 2;                 // K or V of a step as MMA operands
-  static constexpr int kRawSide = U8 ? kChunkTokens * D : kSide;     // as cached
-  static constexpr int kScales = U8 ? 2 * kChunkTokens * 4 : 0;      // row scales of K, then of V
+  static constexpr int kRawSide = TIER == kChunkBytes ? kChunkTokens * D : TIER == kChunkQ4 ? kChunkTokens * (D / 32) * 18 : kSide;  // as cached
+  static constexpr int kScales = TIER == kChunkBytes ? 2 * kChunkTokens * 4 : 0;  // row scales of K, then of V
   static constexpr int kStage = 2 * kRawSide + kScales;
-  static constexpr size_t kSmemBytes = 2 * (size_t)kStage + (U8 ? 2 * kSide : 0);
+  static constexpr size_t kSmemBytes = 2 * (size_t)kStage + (TIER != kChunkHalves ? 2 * kSide : 0);
 };
 
 __device__ __forceinline__ void cp_async16_or_zero(void* smem_dst, const void* gmem_src, bool live) {
@@ -1017,9 +1009,54 @@ __device__ __forceinline__ void cp_async16_or_zero(void* smem_dst, const void* g
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(gmem_src), "r"(live ? 16 : 0));
 }
 
-template <int D, bool BF16, bool U8>
-__global__ void __launch_bounds__(128, U8 ? 2 : 3) attention_chunk_kernel(AttnArgs a) {
-  using Cfg = ChunkCfg<D, U8>;
+// The 4-bit tier's rows (kv_q4.cuh) as f16 values in the operand layout. Rows outside [begin, end) of the page positions that start at
+// `base` come out as zeros of V, whatever they hold.
+template <int D>
+__device__ __forceinline__ void widen_q4_step(const unsigned char* raw, unsigned char* wide, int base, int begin, int end) {
+  constexpr int NB = D / 32, RECORD = kPageTokens * NB * 18, CODES = kPageTokens * D / 2, SIDE = kChunkTokens * D * 2;
+  auto two = [](uint32_t w, bool low) {  // bits 0-3 or 4-7 of both halves -> codes less 8
+    uint32_t bits = (w & (low ? 0x000F000Fu : 0x00F000F0u)) | 0x64006400u;
+    const __half2 h = *reinterpret_cast<__half2*>(&bits);
+    return low ? __hsub2(h, __floats2half2_rn(1032.0f, 1032.0f)) : __hfma2(h, __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-72.0f, -72.0f));
+  };
+  auto word = [](__half2 h) { return *reinterpret_cast<uint32_t*>(&h); };
+  for (int i = threadIdx.x; i < kChunkTokens * 4 * NB; i += 128) {  // a K word: eight values
+    const int row = i / (4 * NB), at = i % (4 * NB), t = at / NB, b = at % NB;
+    const unsigned char* record = raw + row / kPageTokens * RECORD;
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(record + row % kPageTokens * (D / 2) + at * 4);
+    const __half2 d = __half2half2(reinterpret_cast<const __half*>(record + CODES)[row % kPageTokens * NB + b]);
+    *reinterpret_cast<uint4*>(wide + swizzled_offset<D>(row, 4 * b + t)) =
+        make_uint4(word(__hmul2(two(w, true), d)), word(__hmul2(two(w, false), d)), word(__hmul2(two(w >> 8, true), d)), word(__hmul2(two(w >> 8, false), d)));
+  }
+  for (int i = threadIdx.x; i < kChunkTokens * (NB / 2); i += 128) {  // two blocks of a V row
+    const int row = i / (NB / 2), pair = i % (NB / 2);
+    const unsigned char* record = raw + (kChunkPages + row / kPageTokens) * RECORD;
+    uint32_t w[8];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) w[g] = *reinterpret_cast<const uint32_t*>(record + row % kPageTokens * (D / 2) + (g * (NB / 2) + pair) * 4);
+    const bool live = base + row >= begin && base + row < end;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int b = 2 * pair + u;
+      const __half2 d = live ? __half2half2(reinterpret_cast<const __half*>(record + CODES)[row % kPageTokens * NB + b]) : __floats2half2_rn(0.0f, 0.0f);
+      uint32_t x[4];  // the block's codes of columns g = 2 q and 2 q + 1 of every eight
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] = __byte_perm(w[2 * q], w[2 * q + 1], u ? 0x7632 : 0x5410);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = word(__hmul2(two(j < 2 ? x[q] : x[q] >> 8, (j & 1) == 0), d));
+        *reinterpret_cast<uint4*>(wide + SIDE + swizzled_offset<D>(row, 4 * b + j)) = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+    }
+  }
+}
+
+template <int D, bool BF16, int TIER>
+__global__ void __launch_bounds__(128, TIER == kChunkHalves ? 3 : 2) attention_chunk_kernel(AttnArgs a) {
+  constexpr bool U8 = TIER == kChunkBytes, Q4 = TIER == kChunkQ4;
+  using Cfg = ChunkCfg<D, TIER>;
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr int CHUNKS = D / 8, KSTEPS = D / 16, DTILES = D / 8, NT = kChunkTokens / 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -1062,7 +1099,7 @@ __global__ void __launch_bounds__(128, U8 ? 2 : 3) attention_chunk_kernel(AttnAr
 #pragma unroll
       for (int c = threadIdx.x; c < PER_PAGE; c += 128) {
         const size_t src = page[p] * page_stride + (size_t)c * 16;
-        const int at = U8 ? (p * PER_PAGE + c) * 16 : swizzled_offset<D>(p * kPageTokens + c / CHUNKS, c % CHUNKS);
+        const int at = U8 || Q4 ? (p * PER_PAGE + c) * 16 : swizzled_offset<D>(p * kPageTokens + c / CHUNKS, c % CHUNKS);
         cp_async16_or_zero(ks + at, kbase + src, live);
         cp_async16_or_zero(vs + at, vbase + src, live);
       }
@@ -1120,6 +1157,13 @@ __global__ void __launch_bounds__(128, U8 ? 2 : 3) attention_chunk_kernel(AttnAr
         *reinterpret_cast<uint4*>(dst + swizzled_offset<D>(row, chunk)) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(dst + swizzled_offset<D>(row, chunk + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
       }
+      __syncthreads();
+      ks_page = wide;
+      vs_page = wide + Cfg::kSide;
+    }
+    if constexpr (Q4) {
+      unsigned char* wide = smem + 2 * Cfg::kStage;
+      widen_q4_step<D>(raw, wide, (first_page + step * kChunkPages) * kPageTokens, begin, end);
       __syncthreads();
       ks_page = wide;
       vs_page = wide + Cfg::kSide;
@@ -1220,10 +1264,10 @@ __global__ void __launch_bounds__(128, U8 ? 2 : 3) attention_chunk_kernel(AttnAr
   }
 }
 
-template <int D, bool BF16, bool U8>
+template <int D, bool BF16, int TIER>
 static cudaError_t launch_attention_chunk_t(const AttnArgs& args, int batch, cudaStream_t stream) {
-  constexpr size_t smem = ChunkCfg<D, U8>::kSmemBytes;
-  auto kernel = attention_chunk_kernel<D, BF16, U8>;
+  constexpr size_t smem = ChunkCfg<D, TIER>::kSmemBytes;
+  auto kernel = attention_chunk_kernel<D, BF16, TIER>;
   const cudaError_t attr = opt_in_shared_memory(kernel, smem);
   if (attr != cudaSuccess) return attr;
   const int tile_tokens = kChunkRows / (args.q_heads / args.kv_heads);
@@ -1234,7 +1278,7 @@ static cudaError_t launch_attention_chunk_t(const AttnArgs& args, int batch, cud
 bool attention_mma_supported(const PoolView& pool, int q_heads, int tokens) {
   const int G = pool.kv_heads > 0 ? q_heads / pool.kv_heads : 0;
   return tokens >= 1 && pool.block_size == kPageTokens && (pool.head_dim == 64 || pool.head_dim == 128) &&
-         (pool.dtype == kKvF16 || pool.dtype == kKvBF16 || pool.dtype == kKvU8) && G >= 1 && G <= 16 && q_heads % pool.kv_heads == 0;
+         (pool.dtype == kKvF16 || pool.dtype == kKvBF16 || pool.dtype == kKvU8 || (pool.dtype == kKvQ4 && tokens > 1)) && G >= 1 && G <= 16 && q_heads % pool.kv_heads == 0;
 }
 
 AttnPlan plan_attention(int batch, int q_heads, int kv_heads, int head_dim, int max_pages, int sm_count) {
@@ -1288,8 +1332,7 @@ cudaError_t launch_attention_mma(const PoolView& pool, const float* q, const Lan
   if (rope) {
     args.qkv = rope->qkv;
     args.sum = rope->sum;
-    args.inv_freq = rope->inv_freq;
-    args.rope_layout = rope->layout;
+    args.rope = rope->rope;
     args.slab[0] = pool.k;
     args.slab[1] = pool.v;
     args.slab_scale[0] = pool.k_scale;
@@ -1310,7 +1353,7 @@ cudaError_t launch_attention_mma(const PoolView& pool, const float* q, const Lan
   auto launch = [&](auto wide, auto bf16, auto u8) {
     constexpr int D = decltype(wide)::value ? 128 : 64;
     constexpr bool BF16 = decltype(bf16)::value, U8 = decltype(u8)::value;
-    if (tokens > 1) return launch_attention_chunk_t<D, BF16, U8>(args, batch, stream);
+    if (tokens > 1) return launch_attention_chunk_t<D, BF16, U8 ? kChunkBytes : kChunkHalves>(args, batch, stream);
     // Longest lanes first from half as many CTAs again as an SM holds at once (by shared memory and registers: two of f16 pages of
     // 128 columns, three of bytes, four of 64 columns), where a CTA has up to 32 pages and more for each such round: finding its
     // lane costs every CTA some two microseconds. Without and with it, lanes of equal length and of 3 to 100 % of the longest (8 heads
@@ -1331,7 +1374,12 @@ cudaError_t launch_attention_mma(const PoolView& pool, const float* q, const Lan
     if (pool.dtype == kKvBF16) return launch(wide, std::true_type(), std::false_type());
     return launch(wide, std::false_type(), std::false_type());
   };
-  e = pool.head_dim == 128 ? dispatch(std::true_type()) : dispatch(std::false_type());
+  if (pool.dtype == kKvQ4) {  // chunks only: one-token steps are attention_q4.cu's
+    if (tokens == 1) return cudaErrorInvalidValue;
+    e = pool.head_dim == 128 ? launch_attention_chunk_t<128, false, kChunkQ4>(args, batch, stream) : launch_attention_chunk_t<64, false, kChunkQ4>(args, batch, stream);
+  } else {
+    e = pool.head_dim == 128 ? dispatch(std::true_type()) : dispatch(std::false_type());
+  }
   if (e != cudaSuccess) return e;
   if (launches) ++*launches;
   if (tokens > 1) return cudaSuccess;
@@ -1362,10 +1410,11 @@ __device__ __forceinline__ void pool_store(const PoolView& p, void* slab, size_t
 // all heads of a row, otherwise dominate (2048 rows x 48 heads: 104 us with one head per CTA).
 template <int HEADS, int GROUPS>
 __global__ void rope_append_kernel(PoolView pool, const float* qkv, const LaneInfo* lanes,
-                                   const int* tables, const double* __restrict__ inv_freq, int layout,
+                                   const int* tables, RopeView rope,
                                    int q_heads, float* q_out, DeferredSum sum) {
   __shared__ double2 angle[GROUPS > 1 ? 64 : 1];  // (sine, cosine) per pair
   __shared__ float red[32];
+  extern __shared__ float q4_rows[];  // 4-bit tier: [GROUPS][D], a row per group on its way into blocks
   chain_release();  // the next kernel of the step may be scheduled; it waits for this one before touching memory
   const int lane_id = blockIdx.y, tok = blockIdx.z, tokens = gridDim.z;
   const int D = pool.head_dim, half = D / 2, heads = q_heads + 2 * pool.kv_heads;
@@ -1374,9 +1423,9 @@ __global__ void rope_append_kernel(PoolView pool, const float* qkv, const LaneIn
   const bool live = pair < half;  // head dims below 64 leave threads of the warp without a pair
   const int j = live ? pair : 0;
   const size_t row = (size_t)lane_id * tokens + tok;
-  const int i0 = layout == 0 ? j : 2 * j, i1 = layout == 0 ? half + j : 2 * j + 1;
+  const int i0 = rope.first(j), i1 = rope.second(j);
   const int head0 = blockIdx.x * HEADS * GROUPS + group;  // this group's heads: head0, head0 + GROUPS, ...
-  const double freq = inv_freq[j];
+  const double freq = rope.inv_freq[j];
   chain_wait();
   // What the angles and the cells of the cache need, then the heads' inputs, then the angles while those are under way.
   const LaneInfo info = lanes[lane_id];
@@ -1413,7 +1462,11 @@ __global__ void rope_append_kernel(PoolView pool, const float* qkv, const LaneIn
     }
   }
   double s = 0.0, c = 1.0;
-  if (group == 0 && (int)blockIdx.x * HEADS * GROUPS < q_heads + pool.kv_heads) sincos((double)pos * freq, &s, &c);
+  if (group == 0 && (int)blockIdx.x * HEADS * GROUPS < q_heads + pool.kv_heads) {
+    sincos((double)pos * freq, &s, &c);
+    s *= rope.magnitude;
+    c *= rope.magnitude;
+  }
   if (GROUPS > 1) {
     if (group == 0 && live) angle[j] = make_double2(s, c);
     __syncthreads();
@@ -1436,7 +1489,7 @@ __global__ void rope_append_kernel(PoolView pool, const float* qkv, const LaneIn
     const int head = head0 + h * GROUPS;
     const bool is_q = head < q_heads, is_k = !is_q && head < q_heads + pool.kv_heads;
     float r0 = in0[h], r1 = in1[h];
-    if (is_q || is_k) {
+    if ((is_q || is_k) && j < rope.rotary_half) {
       const double first = (double)r0, second = (double)r1;
       r0 = (float)__dsub_rn(__dmul_rn(first, c), __dmul_rn(second, s));
       r1 = (float)__dadd_rn(__dmul_rn(second, c), __dmul_rn(first, s));
@@ -1452,6 +1505,25 @@ __global__ void rope_append_kernel(PoolView pool, const float* qkv, const LaneIn
     const int kv_head = is_k ? head - q_heads : head - q_heads - pool.kv_heads;
     const size_t dst = cached ? pool_elem(pool, page, kv_head, slot) : 0;
     void* slab = is_k ? pool.k : pool.v;
+    if (pool.dtype == kKvQ4) {
+      if (HEADS * GROUPS == 1 && !cached) return;  // as for the int8 tier below
+      float* mine = q4_rows + group * D;
+      if (h > 0) __syncthreads();  // the previous head's rows have been read
+      if (live) {
+        mine[i0] = r0;
+        mine[i1] = r1;
+      }
+      __syncthreads();
+      if (pair < (D / 8 + 31) / 32 * 32) {  // whole warps: four threads to a block
+        const bool stores = cached && pair < D / 8;
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = stores ? mine[pair * 8 + u] : 0.0f;
+        const Q4Row row = stores ? q4_row(pool, slab, page, kv_head, slot) : Q4Row();
+        q4_store_block(v, !is_k, row, pair / 4, D / 32, stores);
+      }
+      continue;
+    }
     if (pool.dtype == kKvU8) {
       // the int8 tier: one scale per cached row, as kv_append_kernel (pool.rs:224-240)
       if (HEADS * GROUPS == 1 && !cached) return;  // the same for the whole CTA; with more heads all threads meet at the barriers
@@ -1481,7 +1553,7 @@ __global__ void rope_append_kernel(PoolView pool, const float* qkv, const LaneIn
 }
 
 cudaError_t launch_rope_append(const PoolView& pool, const float* qkv, const LaneInfo* lanes, const int* tables,
-                               const double* inv_freq, int layout, int batch, int q_heads, float* q_out,
+                               const RopeView& rope, int batch, int q_heads, float* q_out,
                                cudaStream_t stream, const DeferredSum* sum, int tokens) {
   if (batch == 0) return cudaSuccess;
   const int heads = q_heads + 2 * pool.kv_heads, width = std::max(32, (pool.head_dim / 2 + 31) / 32 * 32);
@@ -1489,8 +1561,9 @@ cudaError_t launch_rope_append(const PoolView& pool, const float* qkv, const Lan
   const bool many = (int64_t)batch * tokens >= 128 && !(sum && sum->splits > 0) && width <= 64;
   const int per = many ? 16 : 1;
   const dim3 grid((unsigned)((heads + per - 1) / per), (unsigned)batch, (unsigned)tokens);
-  return launch_chained(many ? rope_append_kernel<4, 4> : rope_append_kernel<1, 1>, grid, dim3((unsigned)(many ? 4 * width : width)), 0, stream, pool, qkv, lanes,
-                        tables, inv_freq, layout, q_heads, q_out, sum ? *sum : DeferredSum());
+  const size_t rows_bytes = pool.dtype == kKvQ4 ? (size_t)(many ? 4 : 1) * pool.head_dim * sizeof(float) : 0;
+  return launch_chained(many ? rope_append_kernel<4, 4> : rope_append_kernel<1, 1>, grid, dim3((unsigned)(many ? 4 * width : width)), rows_bytes, stream, pool, qkv, lanes,
+                        tables, rope, q_heads, q_out, sum ? *sum : DeferredSum());
 }
 
 __global__ void record_step_kernel(const uint32_t* tokens, uint32_t* ids,

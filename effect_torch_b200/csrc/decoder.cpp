@@ -20,6 +20,7 @@
 #include "common.h"
 #include "kernels.h"
 #include "pool.h"
+#include "rotary.h"
 #include "tensor_parallel.h"
 #include "weights.h"
 
@@ -48,7 +49,11 @@ struct etc_decoder {
   std::vector<BoundWeight> attn_norm, ffn_norm, wq, wk, wv, wo, gate, up, down;
   std::vector<etc_qweight*> t_qkv, t_o, t_gu, t_down;
   etc_qweight* t_head = nullptr;
-  double* d_inv_freq = nullptr;
+  double* d_inv_freq = nullptr;  // [head_dim / 2], zeros behind the rotated pairs
+  bool own_rope = false;         // etc_decoder_set_rope: `rope` and its frequencies stand for cfg's theta and layout
+  etc_rope_config rope{};
+  std::vector<double> rope_inv_freq;
+  double rope_magnitude = 1.0;
 
   // device workspaces
   float *hidden = nullptr, *normed = nullptr, *qkv = nullptr, *qr = nullptr, *attl = nullptr, *proj = nullptr, *g = nullptr, *u = nullptr, *act = nullptr,
@@ -84,6 +89,8 @@ struct etc_decoder {
   size_t h_logits_bytes = 0;
   int launches_last_step = 0;
   uint64_t weight_bytes = 0, workspace_bytes = 0;
+  unsigned char* score_buffer = nullptr;  // of etc_decoder_score, made by its first call
+  size_t score_bytes = 0;
 
   cudaGraphExec_t step_graph = nullptr;  // generate_greedy's one-token step
   // what the captured graph baked in: it is re-captured when any of these changes
@@ -126,6 +133,11 @@ int decoder_max_blocks(const etc_decoder_config& c, int max_advance) {
 // covers the longest possible table rounded up the same way.
 size_t decoder_attention_reserve(const etc_decoder_config& c, int max_advance, int sm_count) {
   const int pages = (decoder_max_blocks(c, max_advance) + 7) / 8 * 8;
+  if (c.kv_dtype == ETC_KV_Q4) {  // not monotonic in the table's length: short tables take no scratch, long ones a part per CTA
+    size_t need = 0;
+    for (int p = 1; p <= pages; ++p) need = std::max(need, plan_attention_q4(c.batch, c.q_heads, c.kv_heads, c.head_dim, p, sm_count).scratch_bytes);
+    return need;
+  }
   return plan_attention_max_scratch(c.batch, c.q_heads, c.kv_heads, c.head_dim, pages, sm_count);
 }
 
@@ -202,6 +214,11 @@ etc_status dalloc(etc_decoder* dec, T** out, size_t count) {
   dec->workspace_bytes += count * sizeof(T);
   *out = (T*)p;
   return ETC_OK;
+}
+
+// The tensor-core kernels serve this many query tokens per lane over this cache.
+bool fast_attention_supported(const PoolView& view, int q_heads, int tokens) {
+  return view.dtype == ETC_KV_Q4 && tokens == 1 ? attention_q4_supported(view, q_heads) : attention_mma_supported(view, q_heads, tokens);
 }
 
 struct StepContext {
@@ -358,8 +375,9 @@ etc_status norm_hand_off(StepContext& s, float* x, const BoundWeight& weight, in
   return ETC_OK;
 }
 
-// Enqueues one invocation (all layers + head + greedy argmax) on the runtime's stream.
-etc_status enqueue_step(StepContext& s) {
+// Enqueues the embedding and all layers on the runtime's stream. `pending`: what the last projection left unsummed (one token per
+// lane; chunks finish the residual stream).
+etc_status enqueue_layers(StepContext& s, DeferredSum& pending) {
   etc_decoder* d = s.dec;
   const etc_decoder_config& c = d->cfg;
   cudaStream_t stream = d->rt->stream;
@@ -379,11 +397,11 @@ etc_status enqueue_step(StepContext& s) {
   ++s.launches;
 
   const bool xh = d->xh_path;  // activations go from kernel to kernel as f16 in the tensor-core operand order
-  DeferredSum pending;  // partials of the last projection onto the residual stream, summed by the next RMSNorm
+  pending = DeferredSum();     // partials of the last projection onto the residual stream, summed by the next RMSNorm
   for (int l = 0; l < c.layers; ++l) {
     const size_t li = (size_t)l;
     const PoolView view = s.pool->view(l);
-    const bool fast_attention = d->tiled && !c.exact && attention_mma_supported(view, Hq, T);
+    const bool fast_attention = d->tiled && !c.exact && fast_attention_supported(view, Hq, T);
     const bool rides_attn = norm_rides(s, rows, d->attn_norm[li], {&d->wq[li], &d->wk[li], &d->wv[li]});
     if (xh) {
       ETC_TRY(norm_hand_off(s, d->hidden, d->attn_norm[li], rows, pending));
@@ -397,14 +415,23 @@ etc_status enqueue_step(StepContext& s) {
     else
       ETC_TRY(project_qkv_raw(s, li, rides_attn ? d->hidden : d->normed, rows, qkvw, rides_attn ? &d->attn_norm[li] : nullptr));
     // one token per lane: the attention kernel rotates and appends on its way in
-    const bool fused_rope = fast_attention && T == 1;
+    const bool q4_step = fast_attention && T == 1 && view.dtype == ETC_KV_Q4;
+    const bool fused_rope = fast_attention && T == 1 && !q4_step;
     const bool exact_step = !fast_attention && T == 1 && qkv_sum.splits == 0 && attention_exact_step_supported(view, B, Hq, s.max_ctx, d->rt->sm_count);
-    const FusedRope rope = {d->qkv, qkv_sum, d->d_inv_freq, c.rope_layout};
+    const RopeView positions = {d->d_inv_freq, d->own_rope ? d->rope.layout : c.rope_layout, d->own_rope ? d->rope.rotary_dim / 2 : D / 2, d->rope_magnitude};
+    const FusedRope rope = {d->qkv, qkv_sum, positions};
     if (!fused_rope && !exact_step) {
-      ETC_CUDA(launch_rope_append(view, d->qkv, d->d_lanes, d->d_tables, d->d_inv_freq, c.rope_layout, B, Hq, d->qr, stream, &qkv_sum, T));
+      ETC_CUDA(launch_rope_append(view, d->qkv, d->d_lanes, d->d_tables, positions, B, Hq, d->qr, stream, &qkv_sum, T));
       ++s.launches;
     }
-    if (fast_attention) {
+    if (q4_step) {
+      const Q4Plan plan = plan_attention_q4(B, Hq, Hkv, D, std::max(1, s.max_pages), d->rt->sm_count);
+      if (plan.scratch_bytes > d->attn_scratch_bytes)
+        return fail(ETC_EXECUTION, "kv attention: the plan for " + std::to_string(s.max_pages) + " pages needs " + std::to_string(plan.scratch_bytes) +
+                                       " bytes of partials, the decoder holds " + std::to_string(d->attn_scratch_bytes));
+      ETC_CUDA(launch_attention_q4(view, d->qr, d->d_lanes, d->d_tables, B, Hq, scale, c.window, xh ? nullptr : d->attl, plan, d->attn_scratch, stream,
+                                   &s.launches, xh ? d->xh_att : nullptr, hand_off_stride(rows)));
+    } else if (fast_attention) {
       const AttnPlan plan = plan_attention(B, Hq, Hkv, D, std::max(1, s.max_pages), d->rt->sm_count);
       if (plan.scratch_bytes > d->attn_scratch_bytes)
         return fail(ETC_EXECUTION, "kv attention: split plan for " + std::to_string(s.max_pages) + " pages needs " +
@@ -413,7 +440,7 @@ etc_status enqueue_step(StepContext& s) {
       ETC_CUDA(launch_attention_mma(view, d->qr, d->d_lanes, d->d_tables, B, Hq, scale, c.window, xh ? nullptr : d->attl, plan,
                                     d->attn_scratch, stream, &s.launches, xh ? d->xh_att : nullptr, hand_off_stride(rows), T, fused_rope ? &rope : nullptr));
     } else if (exact_step) {
-      ETC_CUDA(launch_attention_exact_step(view, d->qkv, d->d_lanes, d->d_tables, d->d_inv_freq, c.rope_layout, B, Hq, scale, c.window, d->attl, s.max_ctx, stream));
+      ETC_CUDA(launch_attention_exact_step(view, d->qkv, d->d_lanes, d->d_tables, positions, B, Hq, scale, c.window, d->attl, s.max_ctx, stream));
       ++s.launches;
     } else {
       ETC_CUDA(launch_attention_exact(view, d->qr, d->d_lanes, d->d_tables, B, Hq, T, scale, c.window, d->attl, d->exact_scratch, s.max_ctx, stream, true));
@@ -453,6 +480,16 @@ etc_status enqueue_step(StepContext& s) {
     ETC_TRY(project_into_hidden(s, d->down[li], d->tiled ? d->t_down[li] : nullptr, d->act, rows, xh ? d->xh_act : nullptr, 1,
                                 xh && !finish ? &pending : nullptr));
   }
+  return ETC_OK;
+}
+
+// The final norm and the head over the last row of every lane, into the decoder's logits.
+etc_status enqueue_head(StepContext& s, DeferredSum& pending) {
+  etc_decoder* d = s.dec;
+  const etc_decoder_config& c = d->cfg;
+  cudaStream_t stream = d->rt->stream;
+  const int B = c.batch, T = s.T;
+  const bool xh = d->xh_path;
   // LastTokenRow, the final norm and the head: each row's norm and each head output stand alone, so only the selected row of
   // each lane goes through them
   float* head_in = d->hidden;
@@ -470,6 +507,18 @@ etc_status enqueue_step(StepContext& s) {
   }
   ETC_TRY(run_linear(s, d->head, d->tiled ? d->t_head : nullptr, rides_head ? head_in : d->normed, B, d->logits, ETC_EPILOGUE_NONE, nullptr,
                      xh ? d->xh_norm : nullptr, nullptr, nullptr, rides_head ? &d->out_norm : nullptr));
+  return ETC_OK;
+}
+
+// Enqueues one invocation (all layers + head + greedy argmax) on the runtime's stream.
+etc_status enqueue_step(StepContext& s) {
+  etc_decoder* d = s.dec;
+  const etc_decoder_config& c = d->cfg;
+  cudaStream_t stream = d->rt->stream;
+  const int B = c.batch;
+  DeferredSum pending;
+  ETC_TRY(enqueue_layers(s, pending));
+  ETC_TRY(enqueue_head(s, pending));
   if (d->vocab_global > 0 && d->tp_world > 1) {
     // vocabulary-parallel head: every rank picks its best row, the ranks exchange (logit, token) pairs over peer memory
     if (!d->tp_peer) return fail(ETC_EXECUTION, "tensor parallel: a vocabulary-parallel head needs the peer exchange regions (etc_decoder_tp_peer_import)");
@@ -482,6 +531,90 @@ etc_status enqueue_step(StepContext& s) {
   } else {
     ETC_CUDA(launch_argmax(d->logits, B, c.vocab, d->d_tokens, d->rt->d_status, stream, nullptr, 0, d->h_tokens));
     ++s.launches;
+  }
+  return ETC_OK;
+}
+
+// What etc_decoder_score asks of a step, in host memory: [active, advance] each, the alternatives [active, advance, top].
+struct ScoreRequest {
+  const uint32_t* targets;
+  float *logprobs, *entropy;
+  int top;
+  uint32_t* top_tokens;
+  float* top_logprobs;
+};
+// Rows whose logits exist at a time (131 MB of a vocabulary of 128256): enough for the large-batch linear to run at its rate.
+constexpr int64_t kScoreRows = 256;
+
+// Device buffers of a scoring step, kept from one to the next: [logits][linear scratch][targets][log probabilities][entropy][top tokens][top].
+struct ScoreBuffers {
+  float* logits;
+  void* scratch;
+  uint32_t* targets;
+  float *logprobs, *entropy;
+  uint32_t* top_tokens;
+  float* top_logprobs;
+};
+etc_status score_buffers(etc_decoder* d, int64_t rows, int top, ScoreBuffers* out) {
+  const int64_t at_once = std::min(std::max<int64_t>(kScoreRows, d->cfg.batch), rows);
+  size_t scratch = 0;
+  if (d->tiled)
+    for (int64_t v : {at_once, rows % at_once}) scratch = std::max(scratch, v > 0 ? tiled_scratch_bytes(d->t_head->tiled, v, d->rt->sm_count) : 0);
+  size_t offsets[7], bytes = 0;
+  const size_t sizes[7] = {(size_t)at_once * d->cfg.vocab * 4, scratch, (size_t)rows * 4, (size_t)rows * 4, (size_t)rows * 4, (size_t)rows * top * 4, (size_t)rows * top * 4};
+  for (int i = 0; i < 7; ++i) {
+    offsets[i] = bytes;
+    bytes += (sizes[i] + 255) & ~(size_t)255;
+  }
+  if (bytes > d->score_bytes) {
+    ETC_CUDA(cudaStreamSynchronize(d->rt->stream));
+    if (d->score_buffer) d->rt->device_free(d->score_buffer);
+    d->score_buffer = nullptr;
+    d->score_bytes = 0;
+    ETC_TRY(d->rt->device_alloc(bytes, (void**)&d->score_buffer));
+    d->score_bytes = bytes;
+  }
+  auto at = [&](int i) { return d->score_buffer + offsets[i]; };
+  *out = {(float*)at(0), at(1), (uint32_t*)at(2), (float*)at(3), (float*)at(4), (uint32_t*)at(5), (float*)at(6)};
+  return ETC_OK;
+}
+
+// Enqueues the layers, then norm, head and log probabilities of the `active` lanes' rows, some at a time.
+etc_status enqueue_score(StepContext& s, int active, const ScoreRequest& request, const ScoreBuffers& buffers) {
+  etc_decoder* d = s.dec;
+  const etc_decoder_config& c = d->cfg;
+  cudaStream_t stream = d->rt->stream;
+  const int64_t rows = (int64_t)active * s.T;
+  ETC_CUDA(cudaMemcpyAsync(buffers.targets, request.targets, (size_t)rows * 4, cudaMemcpyHostToDevice, stream));
+  DeferredSum pending;
+  ETC_TRY(enqueue_layers(s, pending));
+  auto score = [&](const float* logits, int64_t row0, int64_t n) -> etc_status {
+    ETC_CUDA(launch_logprobs(logits, n, c.vocab, c.vocab, buffers.targets + row0, buffers.logprobs + row0, buffers.entropy + row0, request.top,
+                             buffers.top_tokens + row0 * request.top, buffers.top_logprobs + row0 * request.top, d->rt->d_status, d->rt->sm_count, stream));
+    ++s.launches;
+    return ETC_OK;
+  };
+  if (s.T == 1) {  // the step's own head
+    ETC_TRY(enqueue_head(s, pending));
+    return score(d->logits, 0, rows);
+  }
+  const int64_t at_once = std::min(std::max<int64_t>(kScoreRows, c.batch), rows);
+  for (int64_t row0 = 0; row0 < rows; row0 += at_once) {
+    const int64_t n = std::min(at_once, rows - row0);
+    float* x = d->hidden + row0 * c.d_model;
+    if (d->xh_path) {
+      ETC_TRY(norm_hand_off(s, x, d->out_norm, n, pending));
+    } else {
+      ETC_CUDA(launch_rmsnorm(x, (const float*)d->out_norm.d_raw, c.rms_eps, n, c.d_model, d->normed, stream));
+      ++s.launches;
+    }
+    if (d->tiled) {
+      ETC_CUDA(launch_qlinear_tiled(d->t_head->tiled, d->normed, n, nullptr, nullptr, ETC_EPILOGUE_NONE, buffers.logits, buffers.scratch, d->rt->d_status,
+                                    d->rt->sm_count, stream, &s.launches, d->xh_path ? d->xh_norm : nullptr, nullptr, hand_off_stride(n)));
+    } else {
+      ETC_TRY(run_linear(s, d->head, nullptr, d->normed, n, buffers.logits, ETC_EPILOGUE_NONE, nullptr));
+    }
+    ETC_TRY(score(buffers.logits, row0, n));
   }
   return ETC_OK;
 }
@@ -620,11 +753,11 @@ bool page_locked(const void* p, size_t bytes) {
 }
 
 bool uses_exact_attention(const etc_decoder* dec, const etc_pool* pool, int T) {
-  return !(dec->tiled && !dec->cfg.exact && attention_mma_supported(pool->view(0), dec->cfg.q_heads, T));
+  return !(dec->tiled && !dec->cfg.exact && fast_attention_supported(pool->view(0), dec->cfg.q_heads, T));
 }
 
 etc_status execute_impl(etc_decoder* dec, etc_pool* pool, etc_seq* const* seqs, int active, const uint32_t* h_tokens, int advance,
-                        float* h_logits, uint32_t* h_out_tokens, const volatile int* cancelled) {
+                        float* h_logits, uint32_t* h_out_tokens, const volatile int* cancelled, const ScoreRequest* request = nullptr) {
   if (!valid_decoder(dec)) return fail(ETC_INVALID_HANDLE, "decoder handle is invalid or destroyed");
   etc_runtime* rt = dec->rt;
   ETC_TRY(activate(rt));
@@ -645,7 +778,26 @@ etc_status execute_impl(etc_decoder* dec, etc_pool* pool, etc_seq* const* seqs, 
   }
   etc_status st = upload_step_inputs(dec);
   if (st != ETC_OK) return abort_with(st);
-  if (advance == 1 && dec->ran_eagerly && !uses_exact_attention(dec, pool, 1)) {
+  std::vector<float> score_results;  // log probabilities, entropy, alternatives' log probabilities, alternatives (bits)
+  if (request) {
+    ScoreBuffers buffers;
+    const int64_t rows = (int64_t)active * advance;
+    st = score_buffers(dec, rows, request->top, &buffers);
+    if (st == ETC_OK) st = enqueue_score(ctx, active, *request, buffers);
+    if (st != ETC_OK) return abort_with(st);
+    score_results.resize((size_t)rows * (2 + 2 * request->top));
+    float* to = score_results.data();
+    cudaError_t ce = cudaSuccess;
+    for (auto [from, n] : {std::pair{(const void*)buffers.logprobs, rows}, std::pair{(const void*)buffers.entropy, rows},
+                           std::pair{(const void*)buffers.top_logprobs, rows * request->top}, std::pair{(const void*)buffers.top_tokens, rows * request->top}}) {
+      if (ce == cudaSuccess && n > 0) ce = cudaMemcpyAsync(to, from, (size_t)n * 4, cudaMemcpyDeviceToHost, rt->stream);
+      to += n;
+    }
+    if (ce != cudaSuccess) {
+      fail(ETC_TRANSFER, std::string("readback failed: ") + cudaGetErrorString(ce));
+      return abort_with(ETC_TRANSFER);
+    }
+  } else if (advance == 1 && dec->ran_eagerly && !uses_exact_attention(dec, pool, 1)) {
     const int bucket = (ctx.max_pages + 7) / 8 * 8;
     if (dec->exec_graph && (dec->exec_graph_active != active || dec->exec_graph_pages != bucket || dec->exec_graph_pool_uid != pool->uid)) {
       cudaGraphExecDestroy(dec->exec_graph);
@@ -723,6 +875,16 @@ etc_status execute_impl(etc_decoder* dec, etc_pool* pool, etc_seq* const* seqs, 
     std::memcpy(h_logits, dec->h_logits, logits_bytes);
   }
   if (h_out_tokens) std::memcpy(h_out_tokens, dec->h_tokens, sizeof(uint32_t) * (size_t)active);
+  if (request) {
+    const size_t rows = (size_t)active * advance, n = rows * request->top;
+    const float* from = score_results.data();
+    std::memcpy(request->logprobs, from, rows * 4);
+    if (request->entropy) std::memcpy(request->entropy, from + rows, rows * 4);
+    if (n > 0) {
+      std::memcpy(request->top_logprobs, from + 2 * rows, n * 4);
+      std::memcpy(request->top_tokens, from + 2 * rows + n, n * 4);
+    }
+  }
   for (int i = 0; i < active; ++i) {
     etc_seq* s = seqs[i];
     const int start = dec->h_lanes[i].start;
@@ -771,7 +933,8 @@ etc_status etc_decoder_create(etc_runtime* rt, const etc_decoder_config* config,
   if (c.max_tokens <= 0 || c.block_size <= 0 || c.max_tokens % c.block_size != 0)  // KvStateSchema::from_native
     return fail(ETC_COMPILATION, "compile: KV max_tokens must be positive and divisible by block_size");
   if (c.batch <= 0) return fail(ETC_COMPILATION, "compile: KV batch must be positive");
-  if (c.kv_dtype < ETC_KV_F32 || c.kv_dtype > ETC_KV_U8) return fail(ETC_COMPILATION, "compile: unsupported KV state dtype");
+  if (c.kv_dtype < ETC_KV_F32 || c.kv_dtype > ETC_KV_Q4) return fail(ETC_COMPILATION, "compile: unsupported KV state dtype");
+  if (c.kv_dtype == ETC_KV_Q4 && c.head_dim % 32 != 0) return fail(ETC_COMPILATION, "compile: the q4 KV state needs a head dim that is a multiple of 32");
   if (c.window != ETC_NO_WINDOW && (c.window <= 0 || c.window > c.max_tokens))
     return fail(ETC_COMPILATION, "compile: KV window must be in 1..=max_tokens");
   etc_decoder* d = new etc_decoder();
@@ -798,6 +961,22 @@ etc_status etc_decoder_set_max_advance(etc_decoder* dec, int max_advance) {
   if (dec->finalized) return fail(ETC_COMPILATION, "compile: the chunk length is fixed once the decoder is finalized");
   if (max_advance <= 0) return fail(ETC_COMPILATION, "compile: chunk length must be positive");
   dec->max_advance = max_advance;
+  return ETC_OK;
+}
+
+etc_status etc_decoder_set_rope(etc_decoder* dec, const etc_rope_config* config, const float* h_divisors) {
+  if (!valid_decoder(dec)) return fail(ETC_INVALID_HANDLE, "decoder handle is invalid or destroyed");
+  if (!config) return fail(ETC_INVALID_ARGUMENT, "rotary: config must not be null");
+  if (dec->finalized) return fail(ETC_COMPILATION, "compile: positions are fixed once the decoder is finalized");
+  if (config->head_dim != dec->cfg.head_dim)
+    return fail(ETC_COMPILATION, "rotary: a head dimension of " + std::to_string(config->head_dim) + " for a decoder of " + std::to_string(dec->cfg.head_dim));
+  std::vector<double> inv_freq;
+  double magnitude = 1.0;
+  ETC_TRY(rope_frequencies(*config, h_divisors, &inv_freq, &magnitude));
+  dec->own_rope = true;
+  dec->rope = *config;
+  dec->rope_inv_freq = std::move(inv_freq);
+  dec->rope_magnitude = magnitude;
   return ETC_OK;
 }
 
@@ -1015,7 +1194,16 @@ etc_status etc_decoder_finalize(etc_decoder* dec) {
     release_raw(dec->head);
   }
   dec->weight_bytes = rt->memory_bytes.load();
-  ETC_TRY(make_inv_freq(rt, c.rope_theta, c.head_dim, &dec->d_inv_freq));
+  if (dec->own_rope) {
+    std::vector<double> table((size_t)c.head_dim / 2, 0.0);
+    std::copy(dec->rope_inv_freq.begin(), dec->rope_inv_freq.end(), table.begin());
+    ETC_TRY(rt->device_alloc(table.size() * sizeof(double), (void**)&dec->d_inv_freq));
+    cudaError_t copied = cudaMemcpyAsync(dec->d_inv_freq, table.data(), table.size() * sizeof(double), cudaMemcpyHostToDevice, rt->stream);
+    if (copied == cudaSuccess) copied = cudaStreamSynchronize(rt->stream);
+    if (copied != cudaSuccess) return fail(ETC_TRANSFER, std::string("rope table upload failed: ") + cudaGetErrorString(copied));
+  } else {
+    ETC_TRY(make_inv_freq(rt, c.rope_theta, c.head_dim, &dec->d_inv_freq));
+  }
 
   const size_t R = (size_t)c.batch * (size_t)dec->max_advance;
   const size_t qw = (size_t)c.q_heads * c.head_dim, kvw = (size_t)c.kv_heads * c.head_dim;
@@ -1102,7 +1290,7 @@ etc_status etc_decoder_destroy(etc_decoder* dec) {
                   (void*)dec->u, (void*)dec->act, (void*)dec->last, (void*)dec->logits, (void*)dec->lin_scratch, (void*)dec->xh_norm,
                   (void*)dec->xh_att, (void*)dec->xh_act,
                   (void*)dec->attn_scratch, (void*)dec->exact_scratch, (void*)dec->d_inputs, (void*)dec->d_tokens,
-                  (void*)dec->d_history, (void*)dec->d_step_counter})
+                  (void*)dec->d_history, (void*)dec->d_step_counter, (void*)dec->score_buffer})
     if (p) rt->device_free(p);
   for (void* p : {(void*)dec->h_inputs, (void*)dec->h_tokens, (void*)dec->h_logits})
     if (p) cudaFreeHost(p);
@@ -1121,6 +1309,22 @@ etc_status etc_decoder_execute_sampled(etc_decoder* dec, etc_pool* pool, etc_seq
                                        const volatile int* cancelled) {
   if (!h_out_tokens) return fail(ETC_INVALID_ARGUMENT, "executeSampled: output token buffer is null");
   return execute_impl(dec, pool, seqs, active, h_tokens, advance, nullptr, h_out_tokens, cancelled);
+}
+
+etc_status etc_decoder_score(etc_decoder* dec, etc_pool* pool, etc_seq* const* seqs, int active, const uint32_t* h_tokens, int advance,
+                             const uint32_t* h_targets, float* h_logprobs, float* h_entropy, int top, uint32_t* h_top_tokens, float* h_top_logprobs,
+                             const volatile int* cancelled) {
+  if (!valid_decoder(dec)) return fail(ETC_INVALID_HANDLE, "decoder handle is invalid or destroyed");
+  if (!h_targets || !h_logprobs || (top > 0 && (!h_top_tokens || !h_top_logprobs)))
+    return fail(ETC_INVALID_ARGUMENT, "score: targets, log probabilities and buffers for the alternatives must be given");
+  if (dec->vocab_global > 0 && dec->tp_world > 1) return fail(ETC_UNSUPPORTED, "score: a vocabulary-parallel head holds a part of every distribution only");
+  ETC_TRY(validate_logprobs(dec->cfg.vocab, top));
+  const bool sized = active >= 0 && active <= dec->cfg.batch && advance >= 0 && advance <= dec->max_advance;  // others are refused below
+  for (int64_t i = 0; sized && i < (int64_t)active * advance; ++i)
+    if (h_targets[i] >= (uint32_t)dec->cfg.vocab)
+      return fail(ETC_INVALID_ARGUMENT, "logprobs: target " + std::to_string(h_targets[i]) + " is outside 0.." + std::to_string(dec->cfg.vocab));
+  const ScoreRequest request = {h_targets, h_logprobs, h_entropy, top, h_top_tokens, h_top_logprobs};
+  return execute_impl(dec, pool, seqs, active, h_tokens, advance, nullptr, nullptr, cancelled, &request);
 }
 
 etc_status etc_decoder_generate_greedy(etc_decoder* dec, etc_pool* pool, etc_seq* const* seqs, int active,

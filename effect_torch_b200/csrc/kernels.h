@@ -217,6 +217,7 @@ cudaError_t launch_sample_rows(const float* logits, int64_t rows, int64_t vocab,
 // Per row of logits: log probability of its target, entropy, the `top` most likely tokens (logprobs.cu). targets with logprobs, and
 // entropy, may be null; top may be 0.
 constexpr int kMaxAlternatives = 32;
+etc_status validate_logprobs(int64_t vocab, int top);  // ops.cpp
 cudaError_t launch_logprobs(const float* logits, int64_t rows, int64_t vocab, int64_t row_stride, const uint32_t* targets, float* logprobs,
                             float* entropy, int top, uint32_t* top_tokens, float* top_logprobs, DeviceStatus* status, int sm_count,
                             cudaStream_t stream);
@@ -264,14 +265,29 @@ AttnPlan plan_attention(int batch, int q_heads, int kv_heads, int head_dim, int 
 // Largest scratch plan_attention can ask for with tables of at most max_pages pages.
 size_t plan_attention_max_scratch(int batch, int q_heads, int kv_heads, int head_dim, int max_pages, int sm_count);
 bool attention_mma_supported(const PoolView& pool, int q_heads, int tokens);
+// Rotary positions of a decoder. Pair j < rotary_half of a head's values turns by position * inv_freq[j] and is scaled by `magnitude`; the
+// values behind the rotated ones pass, as pairs of their own.
+struct RopeView {
+  const double* inv_freq;  // [head_dim / 2], zeros behind rotary_half
+  int layout, rotary_half;
+  double magnitude;
+#ifdef __CUDACC__
+  __device__ __forceinline__ int first(int j) const { return layout == 0 && j < rotary_half ? j : 2 * j; }
+  __device__ __forceinline__ int second(int j) const { return layout == 0 && j < rotary_half ? rotary_half + j : 2 * j + 1; }
+  __device__ __forceinline__ double2 angle(int position, int j) const {  // sine, cosine
+    double s, c;
+    sincos((double)position * inv_freq[j], &s, &c);
+    return make_double2(s * magnitude, c * magnitude);
+  }
+#endif
+};
 // For a decode step: q is not given but comes from the fused projection's rows (or their partials), RoPE and the append of the
 // new token's K and V happen in the attention kernel. Everything else that the kernel reads (cached rows, lanes, tables) must
 // have been written before the launches of this step.
 struct FusedRope {
   const float* qkv;
   DeferredSum sum;
-  const double* inv_freq;
-  int layout;
+  RopeView rope;
 };
 cudaError_t launch_attention_mma(const PoolView& pool, const float* q, const LaneInfo* lanes, const int* tables,
                                  int batch, int q_heads, double scale, long long op_window, float* out,
@@ -280,12 +296,12 @@ cudaError_t launch_attention_mma(const PoolView& pool, const float* q, const Lan
 // RoPE, append and reference-order attention of a decode step (f32 cache, contexts of at most max_ctx in shared memory). As with
 // FusedRope, all it reads but qkv must have been written before the launches of this step.
 bool attention_exact_step_supported(const PoolView& pool, int batch, int q_heads, int max_ctx, int sm_count);
-cudaError_t launch_attention_exact_step(const PoolView& pool, const float* qkv, const LaneInfo* lanes, const int* tables, const double* inv_freq, int layout,
+cudaError_t launch_attention_exact_step(const PoolView& pool, const float* qkv, const LaneInfo* lanes, const int* tables, const RopeView& rope,
                                         int batch, int q_heads, double scale, long long op_window, float* out, int max_ctx, cudaStream_t stream);
 // Fused RoPE(q), RoPE(k) and KV append: qkv [B * tokens, (Hq+2*Hkv)*D] f32 (the fused projection output) ->
 // q_out [B, tokens, Hq, D] f32 rotated, K/V rows written to the pool at positions cursor .. cursor + tokens - 1.
 cudaError_t launch_rope_append(const PoolView& pool, const float* qkv, const LaneInfo* lanes, const int* tables,
-                               const double* inv_freq, int layout, int batch, int q_heads, float* q_out,
+                               const RopeView& rope, int batch, int q_heads, float* q_out,
                                cudaStream_t stream, const DeferredSum* sum = nullptr, int tokens = 1);
 // Tail of a device-resident greedy step: feeds the sampled tokens back as the next ids, appends
 // them to the history, and advances every live lane's cursor (and window start) by one.

@@ -3,6 +3,8 @@ packages/backend-cpu/src/internal/native-addon.ts:316-325."""
 from __future__ import annotations
 
 import ctypes as C
+import math
+import warnings
 from dataclasses import dataclass
 
 import numpy as np
@@ -133,12 +135,42 @@ def llama_geometry(f: GgufFile) -> dict:
                 rope_theta=float(meta.get(f"{arch}.rope.freq_base", 10000.0)))
 
 
+def llama_rope(f: GgufFile, geometry: dict, layout: int):
+    """How a Llama-family file has its positions rotated, as a RopeConfig: `<arch>.rope.dimension_count` (part of the head) and the
+    `<arch>.rope.scaling.*` keys (none, linear, yarn). None where it asks for nothing beyond whole heads at freq_base; a kind of scaling
+    that is not known, or lacks what it needs, is left out with a warning. (The llama3 rule comes as divisors per pair, in the tensor
+    rope_freqs.weight.)"""
+    from . import rope_config
+
+    meta = {m["key"]: m.get("value") for m in f.metadata if not m["array"]}
+    key = lambda name, default=None: meta.get(f"{f.architecture}.rope.{name}", default)
+    rule = {}
+    rotary = int(key("dimension_count", geometry["head_dim"]))
+    if rotary != geometry["head_dim"]:
+        rule["rotary_dim"] = rotary
+    kind = key("scaling.type", "linear" if key("scale_linear") is not None else "none")
+    factor = float(key("scaling.factor", key("scale_linear", 1.0))) or 1.0  # 0: not set
+    original = float(key("scaling.original_context_length", meta.get(f"{f.architecture}.context_length", 0)))
+    if kind == "linear" and factor != 1.0:
+        rule.update(scaling="linear", factor=factor)
+    elif kind == "yarn" and original > 0:
+        rule.update(scaling="yarn", factor=factor, original_context=original)
+        for name, option in (("scaling.yarn_beta_fast", "beta_fast"), ("scaling.yarn_beta_slow", "beta_slow")):
+            if key(name) is not None:
+                rule[option] = float(key(name))
+        attention = float(key("scaling.attn_factor", 1.0))  # on top of the rule's own
+        rule["attention_factor"] = attention * (0.1 * math.log(factor) + 1.0) if attention != 1.0 else 0.0
+    elif kind not in ("none", "linear"):
+        warnings.warn(f"gguf: rope scaling {kind!r} is not known or lacks its original context length; positions are not scaled", stacklevel=3)
+    return rope_config(geometry["head_dim"], theta=geometry["rope_theta"], layout=layout, **rule) if rule else None
+
+
 def load_llama_decoder(rt, path: str, *, batch: int, max_tokens: int, block_size: int = 16, kv_dtype=None, exact: bool = False,
                        max_advance: int = 1, rope_layout=None, window=None):
     """Builds an `Executable` whose weights are streamed from `path` into device memory (packed tensors stay packed and are
     re-tiled on the device at finalize). Tensors: token_embd, blk.N.{attn_norm, attn_q, attn_k, attn_v, attn_output,
-    ffn_norm, ffn_gate, ffn_up, ffn_down}, output_norm, output (falls back to token_embd when the head is tied).
-    Returns (executable, geometry)."""
+    ffn_norm, ffn_gate, ffn_up, ffn_down}, output_norm, output (falls back to token_embd when the head is tied), rope_freqs (frequency
+    divisors). Positions are rotated as the file says (llama_rope). Returns (executable, geometry)."""
     import torch
 
     from . import HALF_SPLIT, KV_F16, W_HEAD, W_OUT_NORM, W_TOK_EMBD, Executable
@@ -146,11 +178,19 @@ def load_llama_decoder(rt, path: str, *, batch: int, max_tokens: int, block_size
     f = GgufFile(path)
     try:
         g = llama_geometry(f)
+        names = {t.name: i for i, t in enumerate(f.tensors)}
+        layout = HALF_SPLIT if rope_layout is None else rope_layout
+        divisors = None
+        if "rope_freqs.weight" in names:
+            info = f.tensors[names["rope_freqs.weight"]]
+            if info.codec != 0:
+                raise BackendError(9, "gguf: rope_freqs.weight must be F32")
+            divisors = f.read_tensor(names["rope_freqs.weight"]).view(np.float32)
         dec = Executable(rt, layers=g["layers"], d_model=g["d_model"], q_heads=g["q_heads"], kv_heads=g["kv_heads"], head_dim=g["head_dim"],
                          ffn=g["ffn"], vocab=g["vocab"], rms_eps=g["rms_eps"], rope_theta=g["rope_theta"],
-                         rope_layout=HALF_SPLIT if rope_layout is None else rope_layout, window=window, batch=batch, max_tokens=max_tokens,
-                         block_size=block_size, kv_dtype=KV_F16 if kv_dtype is None else kv_dtype, exact=exact, max_advance=max_advance)
-        names = {t.name: i for i, t in enumerate(f.tensors)}
+                         rope_layout=layout, window=window, batch=batch, max_tokens=max_tokens, block_size=block_size,
+                         kv_dtype=KV_F16 if kv_dtype is None else kv_dtype, exact=exact, max_advance=max_advance, rope=llama_rope(f, g, layout),
+                         rope_divisors=divisors)
 
         def bind(slot, layer, name):
             if name not in names:

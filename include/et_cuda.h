@@ -528,6 +528,9 @@ ETC_API etc_status etc_decoder_set_weight_device(etc_decoder* dec, etc_weight_sl
  * reference compiles one program per chunk shape ([1,prefillChunk], [1,1], [batch,1],
  * packages/core/src/Model.ts:1906-1946); here one decoder serves every advance up to this bound. */
 ETC_API etc_status etc_decoder_set_max_advance(etc_decoder* dec, int max_advance);
+/* Positions by a rule of their own instead of config.rope_theta and config.rope_layout (see etc_rope_frequencies), before
+ * etc_decoder_finalize: scaled frequencies, part of a head, divisors per pair. config->head_dim is the decoder's. */
+ETC_API etc_status etc_decoder_set_rope(etc_decoder* dec, const etc_rope_config* config, const float* h_divisors);
 /* Freeze the plan: fuse q/k/v and gate/up matrices, size workspaces. */
 ETC_API etc_status etc_decoder_finalize(etc_decoder* dec);
 
@@ -544,6 +547,14 @@ ETC_API etc_status etc_decoder_execute(etc_decoder* dec, etc_pool* pool, etc_seq
 ETC_API etc_status etc_decoder_execute_sampled(etc_decoder* dec, etc_pool* pool, etc_seq* const* seqs, int active,
                                                const uint32_t* h_tokens, int advance, uint32_t* h_out_tokens,
                                                const volatile int* cancelled);
+/* Scores a text: a step like etc_decoder_execute's (any advance up to the chunk length, same transaction) that returns, for every token
+ * fed, the log probability of h_targets [active, advance] (the token that follows it) as etc_logprobs_into defines it, the entropy
+ * (h_entropy may be NULL) and the `top` (0..32) most likely tokens [active, advance, top]. Norm and head run over all rows, some 256 at a
+ * time, in a buffer that the first call makes. Results are written by steps that commit only. A vocabulary-parallel head is
+ * ETC_UNSUPPORTED; a target outside the vocabulary is ETC_INVALID_ARGUMENT before any work. */
+ETC_API etc_status etc_decoder_score(etc_decoder* dec, etc_pool* pool, etc_seq* const* seqs, int active, const uint32_t* h_tokens,
+                                     int advance, const uint32_t* h_targets, float* h_logprobs, float* h_entropy, int top,
+                                     uint32_t* h_top_tokens, float* h_top_logprobs, const volatile int* cancelled);
 /* Device-resident variant for benchmarking the kernel schedule alone: runs `steps` greedy decode
  * steps back to back feeding each step's tokens to the next, without host round trips in between;
  * h_out_tokens [steps, active]. Commits every step. */

@@ -624,6 +624,7 @@ extern "C" {
         columns: i64,
     ) -> EtcStatus;
     pub fn etc_decoder_set_max_advance(dec: *mut EtcDecoder, max_advance: c_int) -> EtcStatus;
+    pub fn etc_decoder_set_rope(dec: *mut EtcDecoder, config: *const EtcRopeConfig, h_divisors: *const f32) -> EtcStatus;
     pub fn etc_decoder_finalize(dec: *mut EtcDecoder) -> EtcStatus;
     pub fn etc_decoder_execute(
         dec: *mut EtcDecoder,
@@ -643,6 +644,21 @@ extern "C" {
         h_tokens: *const u32,
         advance: c_int,
         h_out_tokens: *mut u32,
+        cancelled: *const c_int,
+    ) -> EtcStatus;
+    pub fn etc_decoder_score(
+        dec: *mut EtcDecoder,
+        pool: *mut EtcPool,
+        seqs: *const *mut EtcSeq,
+        active: c_int,
+        h_tokens: *const u32,
+        advance: c_int,
+        h_targets: *const u32,
+        h_logprobs: *mut f32,
+        h_entropy: *mut f32,
+        top: c_int,
+        h_top_tokens: *mut u32,
+        h_top_logprobs: *mut f32,
         cancelled: *const c_int,
     ) -> EtcStatus;
     pub fn etc_decoder_generate_greedy(
