@@ -85,19 +85,25 @@ __device__ __forceinline__ void q4_store_block(const float (&v)[8], bool is_v, c
   if (live && t == 0) row.scales[b] = __float2half_rn(d);
 }
 
-// The reverse: elements 8 t .. 8 t + 7 of block b.
-__device__ __forceinline__ void q4_load_block(const Q4Row& row, bool is_v, int b, int nb, bool live, float (&v)[8]) {
+// The reverse in two halves: what a lane fetches of block b, and elements 8 t .. 8 t + 7 of it.
+struct Q4Part {
+  uint32_t word;
+  float scale;
+};
+__device__ __forceinline__ Q4Part q4_fetch(const Q4Row& row, bool is_v, int b, int nb) {
   const int t = threadIdx.x & 3;
   const uint16_t* src = reinterpret_cast<const uint16_t*>(row.codes);
   const int at = is_v ? 2 * t * nb + b : 2 * (t * nb + b), next = is_v ? at + nb : at + 1;
-  const uint32_t word = live ? src[at] | (uint32_t)src[next] << 16 : 0u;
-  const float d = live ? __half2float(row.scales[b]) : 0.0f;
+  return {src[at] | (uint32_t)src[next] << 16, __half2float(row.scales[b])};
+}
+__device__ __forceinline__ void q4_unpack(const Q4Part& part, bool is_v, float (&v)[8]) {
+  const int t = threadIdx.x & 3;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     uint32_t code;
-    if (is_v) code = __shfl_sync(0xffffffffu, word, i >> 1, 4) >> (4 * t + 16 * (i & 1));
-    else code = word >> (4 * (i >> 1) + 16 * (i & 1));
-    v[i] = __fmul_rn((float)((int)(code & 15u) - 8), d);
+    if (is_v) code = __shfl_sync(0xffffffffu, part.word, i >> 1, 4) >> (4 * t + 16 * (i & 1));
+    else code = part.word >> (4 * (i >> 1) + 16 * (i & 1));
+    v[i] = __fmul_rn((float)((int)(code & 15u) - 8), part.scale);
   }
 }
 

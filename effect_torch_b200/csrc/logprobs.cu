@@ -6,7 +6,7 @@
 //
 // A row is read once. Every thread carries (m, s, t) of its values, rescaled when its maximum rises, and the triples are merged by
 // shuffles, through shared memory and, where several CTAs share a row, through the cluster's. The alternatives need no second
-// pass either: the n-th largest of the 32 half-warps' maxima (a 64-bit key of value and inverted token, so that no two are
+// pass either: the n-th largest of the maxima of 32 groups of threads (a 64-bit key of value and inverted token, so that no two are
 // equal) is a lower bound of the n-th largest key. Only threads whose own maximum reaches it can hold an alternative; a warp
 // looks at each such thread's values again (some hundred, from L2), lists those that reach the bound, and the list is ranked by
 // counting. Should the list overflow (an order of logits made for it), the alternatives are found one after the other instead.
@@ -26,11 +26,9 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kGroups = kThreads / 16;    // half-warps: as many as alternatives can be asked for
-constexpr int kBatch = 4;                 // 16-byte loads in flight per thread
-constexpr int kListed = 2048;             // fewer groups than alternatives hold at most 31 * 16 * 4 values between them
+constexpr int kGroups = 32;               // groups of neighbouring threads: as many as alternatives can be asked for
+constexpr int kBatch = 6;                 // 16-byte loads in flight per thread
+constexpr int kListed = 2048;             // fewer groups than alternatives hold at most 31 * 16 * 4 values between them, of 512 threads
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNothing = -200.0f;       // exp2(kNothing * log2 e) is 0 in f32
@@ -90,9 +88,14 @@ struct Moments {
   }
 };
 
+constexpr long long kNone = 0x7fffffffffffffffll;
+
+template <int THREADS>
 struct Shared {
-  float warp_max[kWarps];
-  double warp_s[kWarps], warp_t[kWarps];
+  float warp_max[THREADS / 32];
+  double warp_s[THREADS / 32], warp_t[THREADS / 32];
+  float row_max;  // the first CTA: of the row
+  double log_s;
   // of the CTA, read by the first of the row's cluster
   float m;
   double s, t;
@@ -101,17 +104,19 @@ struct Shared {
   uint64_t bound;
   uint64_t best[kMaxAlternatives];  // the CTA's alternatives, largest first; 0 where there are none left
   int listed, threads_listed;
-  uint64_t round_best[kWarps];
+  uint64_t round_best[THREADS / 32];
 };
-struct SharedTop : Shared {
+template <int THREADS>
+struct SharedTop : Shared<THREADS> {
   uint64_t list[kListed];
-  short thread_list[kThreads];
+  short thread_list[THREADS];
   uint64_t merged[kMaxCluster * kMaxAlternatives];  // the first CTA: everybody's
 };
 
-template <bool TOP>
-__global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(LogprobArgs a) {
-  using Sh = std::conditional_t<TOP, SharedTop, Shared>;
+template <bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(LogprobArgs a) {
+  constexpr int kThreads = THREADS, kWarps = THREADS / 32, kWidth = THREADS / kGroups;
+  using Sh = std::conditional_t<TOP, SharedTop<THREADS>, Shared<THREADS>>;
   __shared__ Sh sh;
   chain_release();  // the next kernel may be scheduled; it waits for this one before touching memory
   chain_wait();
@@ -132,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(LogprobArgs a) {
     return make_float4(at(i), at(i + 1), at(i + 2), at(i + 3));
   };
   if (threadIdx.x == 0) {
-    sh.bad = 0x7fffffffffffffffll;
+    sh.bad = kNone;
     sh.listed = sh.threads_listed = 0;
   }
   if (TOP) {
@@ -224,11 +229,11 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(LogprobArgs a) {
     own_key = any ? order_key(own_best, at_best) : 0;
     uint64_t group_key = own_key;
 #pragma unroll
-    for (int off = 8; off > 0; off >>= 1) {
+    for (int off = kWidth / 2; off > 0; off >>= 1) {
       const uint64_t o = __shfl_xor_sync(0xffffffffu, group_key, off);
       group_key = o > group_key ? o : group_key;
     }
-    if ((lane & 15) == 0) sh.group_best[threadIdx.x >> 4] = group_key;
+    if (threadIdx.x % kWidth == 0) sh.group_best[threadIdx.x / kWidth] = group_key;
   }
   __syncthreads();
   if (warp == 0) {
@@ -242,6 +247,7 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(LogprobArgs a) {
     if constexpr (TOP) {
       const uint64_t key = sh.group_best[lane];
       int before = 0;
+#pragma unroll
       for (int j = 0; j < kGroups; ++j) {
         const uint64_t o = sh.group_best[j];
         before += o > key || (o == key && j < lane);  // groups without values are equal
@@ -279,7 +285,8 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(LogprobArgs a) {
       for (int k = threadIdx.x; k < listed; k += kThreads) {
         const uint64_t key = sh.list[k];
         int before = 0;
-        for (int j = 0; j < listed && before < a.top; ++j) before += sh.list[j] > key;
+#pragma unroll 8
+        for (int j = 0; j < listed; ++j) before += sh.list[j] > key;
         if (before < a.top) sh.best[before] = key;
       }
     } else {
@@ -306,56 +313,66 @@ __global__ void __launch_bounds__(kThreads, 2) logprobs_kernel(LogprobArgs a) {
   if (cluster.num_blocks() > 1) cluster.sync();
   else __syncthreads();
   if (rank == 0) {
-    float row_max = sh.m;
-    double s = sh.s, t = sh.t;
-    long long bad = sh.bad;
-    for (unsigned r = 1; r < cluster.num_blocks(); ++r) row_max = fmaxf(row_max, cluster.map_shared_rank(&sh, r)->m);
-    if (cluster.num_blocks() > 1) {
-      s = t = 0.0;
-      for (unsigned r = 0; r < cluster.num_blocks(); ++r) {
-        const Sh* peer = cluster.map_shared_rank(&sh, r);
-        if (peer->m > -INFINITY) {
-          const double d = (double)peer->m - (double)row_max, f = exp(d);
-          s += peer->s * f;
-          t += (peer->t + d * peer->s) * f;
-        }
-        bad = min(bad, peer->bad);
-      }
+    const int peers = (int)cluster.num_blocks();
+    if constexpr (TOP) {  // everybody's alternatives are on their way while the sums are put together
+      for (int i = threadIdx.x; i < peers * a.top; i += kThreads) sh.merged[i] = cluster.map_shared_rank(&sh, i / a.top)->best[i % a.top];
     }
-    const double log_s = log(s);
-    if (threadIdx.x == 0) {
-      if (a.entropy) a.entropy[row] = (float)(log_s - t / s);
-      if (a.logprobs) {
-        const uint32_t target = a.targets[row];
-        const bool inside = target < a.vocab;
-        a.logprobs[row] = inside ? (float)(((double)x[target] - (double)row_max) - log_s) : NAN;
-        if (!inside && atomicCAS(&a.status->code, kStatusNone, kStatusTargetOutOfRange) == kStatusNone) {
-          a.status->value = target;
-          a.status->bound = a.vocab;
-        }
+    if (warp == 0) {  // a lane per CTA of the row
+      const bool there = lane < peers;
+      const Sh* peer = cluster.map_shared_rank(&sh, there ? lane : 0);
+      const float peer_m = there ? peer->m : -INFINITY;
+      long long bad = there ? peer->bad : kNone;
+      float row_max = peer_m;
+#pragma unroll
+      for (int off = kMaxCluster / 2; off > 0; off >>= 1) row_max = fmaxf(row_max, __shfl_xor_sync(0xffffffffu, row_max, off));
+      double s = 0.0, t = 0.0;
+      if (peer_m > -INFINITY) {
+        const double d = (double)peer_m - (double)row_max, f = peers > 1 ? exp(d) : 1.0;
+        s = peer->s * f;
+        t = (peer->t + d * peer->s) * f;
       }
-      if (bad != 0x7fffffffffffffffll && atomicCAS(&a.status->code, kStatusNone, kStatusBadLogprobLogit) == kStatusNone) {
-        a.status->value = bad;
-        a.status->bound = row;
+#pragma unroll
+      for (int off = kMaxCluster / 2; off > 0; off >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, off);
+        t += __shfl_xor_sync(0xffffffffu, t, off);
+        bad = min(bad, __shfl_xor_sync(0xffffffffu, bad, off));
+      }
+      if (lane == 0) {
+        const double log_s = log(s);
+        sh.row_max = row_max;
+        sh.log_s = log_s;
+        if (a.entropy) a.entropy[row] = (float)(log_s - t / s);
+        if (a.logprobs) {
+          const uint32_t target = a.targets[row];
+          const bool inside = target < a.vocab;
+          a.logprobs[row] = inside ? (float)(((double)x[target] - (double)row_max) - log_s) : NAN;
+          if (!inside && atomicCAS(&a.status->code, kStatusNone, kStatusTargetOutOfRange) == kStatusNone) {
+            a.status->value = target;
+            a.status->bound = a.vocab;
+          }
+        }
+        if (bad != kNone && atomicCAS(&a.status->code, kStatusNone, kStatusBadLogprobLogit) == kStatusNone) {
+          a.status->value = bad;
+          a.status->bound = row;
+        }
       }
     }
     if constexpr (TOP) {
-      const int n = (int)cluster.num_blocks() * a.top;
-      auto store = [&](int at, uint64_t key) {
-        const size_t o = (size_t)row * a.top + at;
-        a.top_tokens[o] = key_token(key);
-        a.top_logprobs[o] = (float)(((double)key_value(key) - (double)row_max) - log_s);
-      };
-      if (cluster.num_blocks() == 1) {
-        if (threadIdx.x < a.top) store(threadIdx.x, sh.best[threadIdx.x]);
-      } else {
-        if (threadIdx.x < n) sh.merged[threadIdx.x] = cluster.map_shared_rank(&sh, threadIdx.x / a.top)->best[threadIdx.x % a.top];
-        __syncthreads();
-        if (threadIdx.x < n) {
-          const uint64_t key = sh.merged[threadIdx.x];
-          int before = 0;
+      __syncthreads();
+      const int n = peers * a.top;
+      if (threadIdx.x < n) {
+        const uint64_t key = sh.merged[threadIdx.x];
+        int before = 0;
+        if (peers == 1) {
+          before = threadIdx.x;  // in order as they are
+        } else {
+#pragma unroll 8
           for (int j = 0; j < n; ++j) before += sh.merged[j] > key;
-          if (key > 0 && before < a.top) store(before, key);
+        }
+        if (key > 0 && before < a.top) {
+          const size_t o = (size_t)row * a.top + before;
+          a.top_tokens[o] = key_token(key);
+          a.top_logprobs[o] = (float)(((double)key_value(key) - (double)sh.row_max) - sh.log_s);
         }
       }
     }
@@ -384,8 +401,10 @@ cudaError_t launch_logprobs(const float* logits, int64_t rows, int64_t vocab, in
   }
   a.chunks = (int)((pieces + ranks - 1) / ranks);
   const dim3 grid((unsigned)(rows * ranks));
-  if (top > 0) return launch_chained_cluster(logprobs_kernel<true>, grid, dim3(kThreads), 0, stream, ranks, a);
-  return launch_chained_cluster(logprobs_kernel<false>, grid, dim3(kThreads), 0, stream, ranks, a);
+  auto launch = [&](auto kernel, int threads) { return launch_chained_cluster(kernel, grid, dim3((unsigned)threads), 0, stream, ranks, a); };
+  // a row of its own: four small CTAs per SM hide one another's starts and ends; a part of a row: the shorter, the sooner
+  if (ranks == 1) return top > 0 ? launch(logprobs_kernel<true, 256>, 256) : launch(logprobs_kernel<false, 256>, 256);
+  return top > 0 ? launch(logprobs_kernel<true, 512>, 512) : launch(logprobs_kernel<false, 512>, 512);
 }
 
 }  // namespace etc
