@@ -48,32 +48,40 @@ __device__ __forceinline__ void q4_store_block(const float (&v)[8], bool is_v, c
     const float o = __shfl_xor_sync(0xffffffffu, extreme, off);
     if (fabsf(o) > fabsf(extreme) || (fabsf(o) == fabsf(extreme) && (t & off))) extreme = o;  // of equals the first
   }
-  const float d = __fmul_rn(extreme, -0.125f), inv = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
-  uint32_t code[8];
+  const float d = __fmul_rn(extreme, -0.125f), inv = d != 0.0f ? __frcp_rn(d) : 0.0f;
+  // The floor of a value in [0, 16) is the low byte of it plus 2^23, rounded down. Codes are shifted and added with the exponent that the
+  // sums have; what the exponents come to is taken off at the end.
+  auto pack = [&](auto shift_of) {
+    constexpr uint32_t kExponent = 0x4B000000u;
+    uint32_t word = 0, extra = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)  // the floor of a value in [0, 16) is the low byte of it plus 2^23, rounded down
-    code[i] = __float_as_uint(__fadd_rd(fminf(fmaxf(__fadd_rn(__fmul_rn(v[i], inv), 8.5f), 0.0f), 15.5f), 8388608.0f)) & 15u;
+    for (int i = 0; i < 8; ++i) {
+      word += __float_as_uint(__fadd_rd(fminf(fmaxf(__fadd_rn(__fmul_rn(v[i], inv), 8.5f), 0.0f), 15.5f), 8388608.0f)) << shift_of(i);
+      extra += kExponent << shift_of(i);
+    }
+    return word - extra;
+  };
   if (is_v) {
     // element 8 t + g is code t of half word g: byte s of a lane's word holds its codes for g = 2 s and 2 s + 1
-    uint32_t mine = 0;
+    const uint32_t mine = pack([](int i) { return 4 * i; });
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mine |= code[i] << (4 * i);
-    uint32_t even = 0, odd = 0;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const uint32_t byte = __shfl_sync(0xffffffffu, mine, s, 4) >> (8 * t);
-      even |= (byte & 15u) << (4 * s);
-      odd |= ((byte >> 4) & 15u) << (4 * s);
-    }
+    for (int s = 0; s < 4; ++s) w[s] = __shfl_sync(0xffffffffu, mine, s, 4);
+    const unsigned pick = (unsigned)(t | (t + 4) << 4);
+    const uint32_t bytes = __byte_perm(__byte_perm(w[0], w[1], pick), __byte_perm(w[2], w[3], pick), 0x5410);
+    auto nibbles = [](uint32_t x) {  // the low ones of the four bytes, side by side
+      x &= 0x0F0F0F0Fu;
+      x |= x >> 4;
+      return __byte_perm(x, 0u, 0x4420) & 0xFFFFu;
+    };
+    const uint32_t even = nibbles(bytes), odd = nibbles(bytes >> 4);
     if (live) {
       uint16_t* dst = reinterpret_cast<uint16_t*>(row.codes);
       dst[2 * t * nb + b] = (uint16_t)even;
       dst[(2 * t + 1) * nb + b] = (uint16_t)odd;
     }
   } else if (live) {
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) word |= code[i] << (4 * (i >> 1) + 16 * (i & 1));
+    const uint32_t word = pack([](int i) { return 4 * (i >> 1) + 16 * (i & 1); });
     uint16_t* dst = reinterpret_cast<uint16_t*>(row.codes) + 2 * (t * nb + b);
     if ((reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
       *reinterpret_cast<uint32_t*>(dst) = word;
@@ -103,7 +111,8 @@ __device__ __forceinline__ void q4_unpack(const Q4Part& part, bool is_v, float (
     uint32_t code;
     if (is_v) code = __shfl_sync(0xffffffffu, part.word, i >> 1, 4) >> (4 * t + 16 * (i & 1));
     else code = part.word >> (4 * (i >> 1) + 16 * (i & 1));
-    v[i] = __fmul_rn((float)((int)(code & 15u) - 8), part.scale);
+    // 2^23 + code less 2^23 + 8: a conversion from integers would take the slowest pipe
+    v[i] = __fmul_rn(__fsub_rn(__uint_as_float((code & 15u) | 0x4B000000u), 8388616.0f), part.scale);
   }
 }
 
