@@ -124,8 +124,29 @@ __device__ __forceinline__ void lane_at(const Q4Args& a, long long at, int units
   *before = base;
 }
 
-__device__ __forceinline__ void copy16(unsigned dst, const uint8_t* src) {  // dst in shared memory
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// A record of K and one of V by a warp, 16 bytes per lane and instruction; `rest`: this lane has some of what is left over 512s.
+template <int RECORD>
+__device__ __forceinline__ void copy_records(unsigned dst, const uint8_t* k, const uint8_t* v, int rest) {
+  static_assert(RECORD == 1152 || RECORD == 576, "16 rows of 128 or 64 values");
+  if constexpr (RECORD == 1152) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t"
+        "cp.async.cg.shared.global [%0], [%1], 16;\n\t"
+        "cp.async.cg.shared.global [%0+512], [%1+512], 16;\n\t"
+        "@p cp.async.cg.shared.global [%0+1024], [%1+1024], 16;\n\t"
+        "cp.async.cg.shared.global [%0+1152], [%2], 16;\n\t"
+        "cp.async.cg.shared.global [%0+1664], [%2+512], 16;\n\t"
+        "@p cp.async.cg.shared.global [%0+2176], [%2+1024], 16;\n\t}" ::"r"(dst), "l"(k), "l"(v), "r"(rest)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\t"
+        "cp.async.cg.shared.global [%0], [%1], 16;\n\t"
+        "@p cp.async.cg.shared.global [%0+512], [%1+512], 16;\n\t"
+        "cp.async.cg.shared.global [%0+576], [%2], 16;\n\t"
+        "@p cp.async.cg.shared.global [%0+1088], [%2+512], 16;\n\t}" ::"r"(dst), "l"(k), "l"(v), "r"(rest)
+        : "memory");
+  }
 }
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -147,6 +168,8 @@ __device__ __forceinline__ float exp2_flushed(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+// A value that all lanes have, as one that the compiler knows them to have.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 halves(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 // Constants of the widening, each in a register of its own: as immediates they would cost an instruction more per use.
@@ -226,7 +249,7 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
   using Cfg = Q4Cfg<D, PAIRS, WARPS>;
   constexpr int NB = Cfg::kBlocks, MINE = PAIRS ? 1 : 2;  // heads whose scores a thread holds: t, or 2 t and 2 t + 1
   extern __shared__ __align__(128) unsigned char smem[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int lane = threadIdx.x & 31, warp = uniform(threadIdx.x >> 5), g = lane >> 2, t = lane & 3;
   const int units = a.kv_heads * a.groups, G = a.q_heads / a.kv_heads;
   chain_release();
   chain_wait();
@@ -234,14 +257,15 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
   Cursor run;
   auto enter = [&](Cursor& c) {  // c.lane, c.unit and c.at are set; page0 relative to the unit's first page
     const LaneInfo info = a.lanes[c.lane];
-    c.span = span_of(info, a.op_window);
-    c.table = info.table_offset;
+    const Span span = span_of(info, a.op_window);
+    c.span = {uniform(span.begin), uniform(span.end), uniform(span.first), uniform(span.pages)};
+    c.table = uniform(info.table_offset);
   };
   // the part of the unit from its place `skipped` on; it may hold no page
   auto clip = [&](Cursor& c, int skipped) {
     const int places = c.span.pages + kUnitPages, upto = (int)min((long long)places, skipped + (c.stop - c.at));
-    c.page0 = c.span.first + max(skipped - kUnitPages, 0);
-    c.page1 = c.span.first + max(upto - kUnitPages, 0);
+    c.page0 = uniform(c.span.first + max(skipped - kUnitPages, 0));
+    c.page1 = uniform(c.span.first + max(upto - kUnitPages, 0));
     c.at += upto - skipped;  // where the next unit begins
   };
   // the next unit of the run of which it has pages; false when there is none
@@ -326,17 +350,15 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
     aim();
     look_up();
   }
+  const int rest = lane * 16 < Cfg::kRecord % 512;
+  auto copy = [&](unsigned offset) {
+    const unsigned long long from = (unsigned long long)ahead_number * page_stride;
+    copy_records<Cfg::kRecord>(ring_at + offset, ahead_k + from, ahead_v + from, rest);
+    ++ahead_page;
+  };
   auto issue = [&](unsigned offset) {
     if (more) {
-      const uint8_t *k = ahead_k + (unsigned long long)ahead_number * page_stride, *v = ahead_v + (unsigned long long)ahead_number * page_stride;
-      const unsigned dst = ring_at + offset;
-#pragma unroll
-      for (int c = 0; c < Cfg::kRecord; c += 512)
-        if (c + 512 <= Cfg::kRecord || lane * 16 + c < Cfg::kRecord) {
-          copy16(dst + c, k + c);
-          copy16(dst + Cfg::kRecord + c, v + c);
-        }
-      ++ahead_page;
+      copy(offset);
       look_up();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -411,8 +433,18 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
     __half2 top_half = __float2half2_rn(top_scale), to_range = scale_to_range(top_scale);
     const int inner0 = (run.span.begin + kPage - 1) / kPage, inner1 = run.span.end / kPage;  // pages without a masked token
 
+    // while the copies are in this unit too, the next number is in its table
+    const bool together = more && ahead.lane == run.lane && ahead.unit == run.unit;
+    const int close = uniform(together ? run.page0 + run.page1 - 1 - ahead_page : run.page0);
+    const int* table = a.tables + run.table;
     for (int page = run.page0; page < run.page1; ++page) {
-      issue(fill);
+      if (page < close) {
+        copy(fill);
+        ahead_number = (unsigned)table[ahead_page];
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      } else {
+        issue(fill);
+      }
       step(fill);
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       __syncwarp();
