@@ -40,7 +40,9 @@ namespace {
 
 constexpr int kPage = 16;
 constexpr int kStages = 3;
-constexpr int kDirectPages = 16;
+// Tables of up to 32 pages take a CTA per unit: 512 tokens of 1, 8 and 32 sequences (8 KV heads of 128) 8.2, 10.4 and 10.9 us against
+// 10.3, 12.0 and 15.2 by runs; 1024 tokens 10.8, 14.5 and 15.0 against 10.7, 12.5 and 17.9.
+constexpr int kDirectPages = 32;
 constexpr int kUnitPages = 6;  // what a unit costs beyond its pages, in pages
 constexpr int kPartPad = 4;  // of a head's part: reference, sum of weights, two unused
 constexpr float kSlack = 6.0f;
