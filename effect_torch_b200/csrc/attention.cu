@@ -147,14 +147,13 @@ __device__ __forceinline__ float exact_load(const void* slab, size_t elem, float
 // Column c of a cached row (row = (page * kv_heads + head) * block_size + slot).
 template <int DTYPE>
 __device__ __forceinline__ float exact_value(const PoolView& p, bool is_v, int row, int c, float scale) {
-  void* slab = is_v ? p.v : p.k;
   if constexpr (DTYPE == kKvQ4) {
     const int record = row / p.block_size;  // pages of one head each
     PoolView records = p;
     records.kv_heads = 1;
-    return q4_value(q4_row(records, slab, record, 0, row - record * p.block_size), is_v, c, p.head_dim / 32);
+    return q4_value(q4_row(records, is_v, record, 0, row - record * p.block_size), is_v, c, p.head_dim / 32);
   }
-  return exact_load<DTYPE>(slab, (size_t)row * p.head_dim + c, scale);
+  return exact_load<DTYPE>(is_v ? p.v : p.k, (size_t)row * p.head_dim + c, scale);
 }
 
 // `tokens_first`: q and out are [B, tokens, Hq, D] (the fused projection's order) instead of [B, Hq, tokens, D].
@@ -1028,16 +1027,16 @@ __device__ __forceinline__ void widen_q4_step(const unsigned char* raw, unsigned
     *reinterpret_cast<uint4*>(wide + swizzled_offset<D>(row, 4 * b + t)) =
         make_uint4(word(__hmul2(two(w, true), d)), word(__hmul2(two(w, false), d)), word(__hmul2(two(w >> 8, true), d)), word(__hmul2(two(w >> 8, false), d)));
   }
-  for (int i = threadIdx.x; i < kChunkTokens * (NB / 2); i += 128) {  // two blocks of a V row
-    const int row = i / (NB / 2), pair = i % (NB / 2);
-    const unsigned char* record = raw + (kChunkPages + row / kPageTokens) * RECORD;
+  for (int i = threadIdx.x; i < kChunkTokens / 2 * NB; i += 128) {  // a block of two V rows, which lie together
+    const int row0 = i / NB * 2, b = i % NB;
+    const unsigned char* record = raw + (kChunkPages + row0 / kPageTokens) * RECORD;
     uint32_t w[8];
 #pragma unroll
-    for (int g = 0; g < 8; ++g) w[g] = *reinterpret_cast<const uint32_t*>(record + row % kPageTokens * (D / 2) + (g * (NB / 2) + pair) * 4);
-    const bool live = base + row >= begin && base + row < end;
+    for (int g = 0; g < 8; ++g) w[g] = *reinterpret_cast<const uint32_t*>(record + row0 % kPageTokens * (D / 2) + (g * NB + b) * 4);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int b = 2 * pair + u;
+      const int row = row0 + u;
+      const bool live = base + row >= begin && base + row < end;
       const __half2 d = live ? __half2half2(reinterpret_cast<const __half*>(record + CODES)[row % kPageTokens * NB + b]) : __floats2half2_rn(0.0f, 0.0f);
       uint32_t x[4];  // the block's codes of columns g = 2 q and 2 q + 1 of every eight
 #pragma unroll
@@ -1519,7 +1518,7 @@ __global__ void rope_append_kernel(PoolView pool, const float* qkv, const LaneIn
         float v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) v[u] = stores ? mine[pair * 8 + u] : 0.0f;
-        const Q4Row row = stores ? q4_row(pool, slab, page, kv_head, slot) : Q4Row();
+        const Q4Row row = stores ? q4_row(pool, !is_k, page, kv_head, slot) : Q4Row();
         q4_store_block(v, !is_k, row, pair / 4, D / 32, stores);
       }
       continue;

@@ -9,19 +9,20 @@
 // Nothing else is below f32.
 //
 // Layout. Tokens are the rows of the first product and the columns of the second: S^T = K Q^T and O^T = V^T P^T. A code page is read from
-// shared memory as it was stored: 16 bytes of a K row per thread are its operands of all eight steps, 8 bytes of a V row its operands of
-// all eight tiles; two codes are widened by one mask and one f16 operation. The eight columns of a tile are the heads of a KV head: up to
+// shared memory as it was stored: 16 bytes of a K row per thread are its operands of all eight steps, 16 bytes of a pair of V rows its
+// operands of all eight tiles; two codes are widened by one mask and one f16 operation. The eight columns of a tile are the heads of a KV head: up to
 // four (PAIRS) as (value, rest) pairs, so that the split costs no tensor instruction where columns would stay empty, and a thread
 // adds the two sums of its head; five to eight as they are, with a second product for the rests onto the same sums.
 //
 // What bounds it is the issue rate, not HBM: some 400 instructions per page and warp, 152 of them widening codes.
 //
 // Work. The pages of all (lane, KV head) units in a row are cut into as many equal runs as there are warps, whatever the lengths of the
-// lanes: nobody waits for the longest. A warp takes its run page by page through a ring of cp.async copies that runs on across units, and
-// writes the units that lie inside it. What neighbouring warps of a CTA have of one unit is added up in shared memory at the end;
+// lanes: nobody waits for the longest. A warp takes its run by pages, or pairs of them, through a ring of cp.async copies that runs on
+// across units, and writes the units that lie inside it. What neighbouring warps of a CTA have of one unit is added up in shared memory at the end;
 // the parts of a unit that several CTAs share go to scratch (two per CTA at most) and a second kernel adds them up. Short tables
 // (kDirectPages) take one CTA per unit and no second kernel. (Runs of whole CTAs, whose warps took pages in turn and met after each
-// unit: 67 us against XX for 64 lanes of 128 to 4096 tokens.)
+// unit: 67 us against 51 for 64 lanes of 128 to 4096 tokens.) With PAIRS a warp has the registers to take two pages at once, whose scores,
+// reference and weights do not wait for each other: 45.8 us against 49.2 by single pages; a ring of two such steps does as well as longer ones.
 //
 // Scores are compared with a reference that is raised, with everything accumulated, only when one exceeds it by 2^kSlack: a few times per
 // run instead of once per page.
@@ -39,9 +40,10 @@ namespace etc {
 namespace {
 
 constexpr int kPage = 16;
-constexpr int kStages = 3;
-// Tables of up to 32 pages take a CTA per unit: 512 tokens of 1, 8 and 32 sequences (8 KV heads of 128) 8.2, 10.4 and 10.9 us against
-// 10.3, 12.0 and 15.2 by runs; 1024 tokens 10.8, 14.5 and 15.0 against 10.7, 12.5 and 17.9.
+constexpr int kStages = 2;
+constexpr int kWarps = 4, kResident = 3;  // of a CTA; CTAs of an SM: 168 registers for a thread
+// Tables of up to 32 pages take a CTA per unit: 512 tokens of 1, 8 and 32 sequences (8 KV heads of 128) 8.3, 10.1 and 11.8 us against
+// 9.7, 11.4 and 17.7 by runs; 1024 tokens 11.2, 15.1 and 17.3 against 10.9, 12.0 and 20.5.
 constexpr int kDirectPages = 32;
 constexpr int kUnitPages = 6;  // what a unit costs beyond its pages, in pages
 constexpr int kPartPad = 4;  // of a head's part: reference, sum of weights, two unused
@@ -151,12 +153,12 @@ __device__ __forceinline__ void copy_records(unsigned dst, const uint8_t* k, con
   }
 }
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {  // onto zeros
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
@@ -211,16 +213,18 @@ __device__ __forceinline__ void store_out(const Q4Args& a, int D, int row, int k
 // What V scales are multiplied by, of which no |dv| exceeds the power of two `top`: 1 / top, as far as f16 holds it.
 __device__ __forceinline__ __half2 scale_to_range(float top) { return __float2half2_rn(fminf(1.0f / top, 32768.0f)); }
 
-template <int D, bool PAIRS, int WARPS>
+template <int D, bool PAIRS>
 struct Q4Cfg {
   static constexpr int kBlocks = D / 32;
   static constexpr int kCodes = kPage * D / 2;                  // code bytes of a record
   static constexpr int kRecord = kCodes + kPage * kBlocks * 2;
-  static constexpr int kStage = 2 * kRecord;                    // K, then V
+  static constexpr int kTogether = PAIRS ? 2 : 1;               // pages that a warp takes at once
+  static constexpr int kBoth = 2 * kRecord;                     // K, then V
+  static constexpr int kStage = kTogether * kBoth;
   static constexpr int kHeads = PAIRS ? 4 : 8;
   static constexpr int kPitch = D + 8;                          // of a head's partial sums: no bank conflicts
-  static constexpr int kRing = WARPS * kStages * kStage;
-  static constexpr size_t kSmem = kRing + (size_t)2 * WARPS * kHeads * (kPitch + 2) * sizeof(float);
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr size_t kSmem = kRing + (size_t)2 * kWarps * kHeads * (kPitch + 2) * sizeof(float);
 };
 
 // N words (1, 2 or 4) from shared memory, aligned to their size.
@@ -246,10 +250,10 @@ struct Cursor {
   int page0, page1;    // this run's pages of the unit (block-table indexes)
 };
 
-template <int D, bool PAIRS, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) attention_q4_kernel(Q4Args a) {
-  using Cfg = Q4Cfg<D, PAIRS, WARPS>;
-  constexpr int NB = Cfg::kBlocks, MINE = PAIRS ? 1 : 2;  // heads whose scores a thread holds: t, or 2 t and 2 t + 1
+template <int D, bool PAIRS>
+__global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4Args a) {
+  using Cfg = Q4Cfg<D, PAIRS>;
+  constexpr int NB = Cfg::kBlocks, PAGES = Cfg::kTogether, MINE = PAIRS ? 1 : 2;  // MINE: heads whose scores a thread holds: t, or 2 t and 2 t + 1
   extern __shared__ __align__(128) unsigned char smem[];
   const int lane = threadIdx.x & 31, warp = uniform(threadIdx.x >> 5), g = lane >> 2, t = lane & 3;
   const int units = a.kv_heads * a.groups, G = a.q_heads / a.kv_heads;
@@ -287,9 +291,9 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
   if (!a.direct) {  // lanes with nothing to attend over
     for (int l = blockIdx.x; l < a.batch; l += gridDim.x)
       if (span_of(a.lanes[l], a.op_window).pages == 0)
-        for (int i = threadIdx.x; i < a.q_heads * D; i += WARPS * 32) store_out(a, D, l, i, 0.0f);
+        for (int i = threadIdx.x; i < a.q_heads * D; i += kWarps * 32) store_out(a, D, l, i, 0.0f);
   }
-  __shared__ Record records[2 * WARPS];  // of each warp the unit that began before its run, the unit that goes on behind it
+  __shared__ Record records[2 * kWarps];  // of each warp the unit that began before its run, the unit that goes on behind it
   if (lane < 2) records[2 * warp + lane].valid = 0;
   bool works = true;
   if (a.direct) {
@@ -298,17 +302,17 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
     enter(run);
     if (run.span.pages == 0) {  // nothing to attend over
       const int kv_head = run.unit / a.groups, head0 = kv_head * G + (run.unit - kv_head * a.groups) * a.heads;
-      for (int i = threadIdx.x; i < min(a.heads, (kv_head + 1) * G - head0) * D; i += WARPS * 32) store_out(a, D, run.lane, head0 * D + i, 0.0f);
+      for (int i = threadIdx.x; i < min(a.heads, (kv_head + 1) * G - head0) * D; i += kWarps * 32) store_out(a, D, run.lane, head0 * D + i, 0.0f);
       return;
     }
-    const int from = run.span.pages * warp / WARPS;
+    const int from = run.span.pages * warp / kWarps;
     run.at = kUnitPages + from;
-    run.stop = kUnitPages + run.span.pages * (warp + 1) / WARPS;
+    run.stop = kUnitPages + run.span.pages * (warp + 1) / kWarps;
     works = run.at < run.stop;
     clip(run, kUnitPages + from);
   } else {
     const long long total = all_places(a) * units;
-    const int runs = (int)gridDim.x * WARPS, mine = (int)blockIdx.x * WARPS + warp;
+    const int runs = (int)gridDim.x * kWarps, mine = (int)blockIdx.x * kWarps + warp;
     const long long begin = total * mine / runs;
     run.stop = total * (mine + 1) / runs;
     works = begin < run.stop;
@@ -331,7 +335,7 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
   const unsigned ring_at = (unsigned)__cvta_generic_to_shared(ring) + lane * 16;
   Cursor ahead = run;
   int ahead_page = run.page0;
-  unsigned ahead_number = 0;
+  unsigned ahead_number[PAGES] = {};
   const uint8_t *ahead_k, *ahead_v;  // page 0 of the unit's KV head, this lane's 16 bytes
   bool more = works;
   const unsigned page_stride = (unsigned)(a.kv_heads * Cfg::kRecord);
@@ -346,7 +350,10 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
       ahead_page = ahead.page0;
       aim();
     }
-    if (more) ahead_number = (unsigned)a.tables[ahead.table + ahead_page];
+    if (!more) return;
+#pragma unroll
+    for (int u = 0; u < PAGES; ++u)  // what lies behind the last page is that page again, and masked
+      ahead_number[u] = (unsigned)a.tables[ahead.table + min(ahead_page + u, ahead.page1 - 1)];
   };
   if (works) {
     aim();
@@ -354,9 +361,12 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
   }
   const int rest = lane * 16 < Cfg::kRecord % 512;
   auto copy = [&](unsigned offset) {
-    const unsigned long long from = (unsigned long long)ahead_number * page_stride;
-    copy_records<Cfg::kRecord>(ring_at + offset, ahead_k + from, ahead_v + from, rest);
-    ++ahead_page;
+#pragma unroll
+    for (int u = 0; u < PAGES; ++u) {
+      const unsigned long long from = (unsigned long long)ahead_number[u] * page_stride;
+      copy_records<Cfg::kRecord>(ring_at + offset + u * Cfg::kBoth, ahead_k + from, ahead_v + from, rest);
+    }
+    ahead_page += PAGES;
   };
   auto issue = [&](unsigned offset) {
     if (more) {
@@ -374,9 +384,8 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
   }
 
   float* sums = reinterpret_cast<float*>(smem + Cfg::kRing);  // [record][head][pitch], then references and weights [record][head]
-  float* refs = sums + 2 * WARPS * Cfg::kHeads * Cfg::kPitch;
-  float* weights = refs + 2 * WARPS * Cfg::kHeads;
-  const int row_lo = (g >> 1) + 4 * (g & 1);  // tokens of this thread's scores, row_lo and row_lo + 8: row r of a tile is token r/2 + 4 (r%2)
+  float* refs = sums + 2 * kWarps * Cfg::kHeads * Cfg::kPitch;
+  float* weights = refs + 2 * kWarps * Cfg::kHeads;
   const Widen widen;
   const bool wide_q = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;
   while (works) {
@@ -433,16 +442,18 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
     for (int i = 0; i < 2 * NB; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
     float top_scale = kSmallestScale;  // power of two that no |dv| so far exceeds
     __half2 top_half = __float2half2_rn(top_scale), to_range = scale_to_range(top_scale);
-    const int inner0 = (run.span.begin + kPage - 1) / kPage, inner1 = run.span.end / kPage;  // pages without a masked token
+    // this run's positions of the unit, and the pages of it without a masked token
+    const int end_of_run = min(run.span.end, run.page1 * kPage), inner0 = (run.span.begin + kPage - 1) / kPage, inner1 = end_of_run / kPage;
 
-    // while the copies are in this unit too, the next number is in its table
+    // while the copies are in this unit too, and whole, the next numbers are in its table
     const bool together = more && ahead.lane == run.lane && ahead.unit == run.unit;
-    const int close = uniform(together ? run.page0 + run.page1 - 1 - ahead_page : run.page0);
+    const int close = uniform(together ? run.page0 + run.page1 - (2 * PAGES - 1) - ahead_page : run.page0);
     const int* table = a.tables + run.table;
-    for (int page = run.page0; page < run.page1; ++page) {
+    for (int page = run.page0; page < run.page1; page += PAGES) {
       if (page < close) {
         copy(fill);
-        ahead_number = (unsigned)table[ahead_page];
+#pragma unroll
+        for (int u = 0; u < PAGES; ++u) ahead_number[u] = (unsigned)table[ahead_page + u];
         asm volatile("cp.async.commit_group;" ::: "memory");
       } else {
         issue(fill);
@@ -450,19 +461,21 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
       step(fill);
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
       __syncwarp();
-      const unsigned char *codes = ring + at + row_lo * (D / 2) + t * (4 * NB), *scales = ring + at + Cfg::kCodes + row_lo * (2 * NB);
+      const unsigned char *codes = ring + at + g * (D / 2) + t * (4 * NB), *scales = ring + at + Cfg::kCodes + g * (2 * NB);
 
-      // scores of tokens row_lo and row_hi
-      float s_lo[MINE], s_hi[MINE];
+      // scores of tokens g and g + 8 of each page
+      float s_lo[PAGES][MINE], s_hi[PAGES][MINE];
+      __align__(8) uint32_t dv_lo[PAGES][NB / 2], dv_hi[PAGES][NB / 2];
 #pragma unroll
-      for (int m = 0; m < MINE; ++m) s_lo[m] = s_hi[m] = 0.0f;
-      {
+      for (int u = 0; u < PAGES; ++u) {
+#pragma unroll
+        for (int m = 0; m < MINE; ++m) s_lo[u][m] = s_hi[u][m] = 0.0f;
         __align__(16) uint32_t w_lo[NB], w_hi[NB];
         __align__(8) uint32_t d_lo[NB / 2], d_hi[NB / 2];
-        load_words<NB>(w_lo, codes);
-        load_words<NB>(w_hi, codes + 8 * (D / 2));
-        load_words<NB / 2>(d_lo, scales);
-        load_words<NB / 2>(d_hi, scales + 8 * (2 * NB));
+        load_words<NB>(w_lo, codes + u * Cfg::kBoth);
+        load_words<NB>(w_hi, codes + u * Cfg::kBoth + 8 * (D / 2));
+        load_words<NB / 2>(d_lo, scales + u * Cfg::kBoth);
+        load_words<NB / 2>(d_hi, scales + u * Cfg::kBoth + 8 * (2 * NB));
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           const uint32_t x = w_lo[b], y = w_hi[b], x8 = x >> 8, y8 = y >> 8;
@@ -474,48 +487,54 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
           mma_first(c, a00, a01, a02, a03, qf[0][b][0][0], qf[0][b][0][1]);
           mma(c, a10, a11, a12, a13, qf[0][b][1][0], qf[0][b][1][1]);
           if constexpr (PAIRS) {
-            s_lo[0] = fmaf(d0, c[0] + c[1], s_lo[0]);
-            s_hi[0] = fmaf(d1, c[2] + c[3], s_hi[0]);
+            s_lo[u][0] = fmaf(d0, c[0] + c[1], s_lo[u][0]);
+            s_hi[u][0] = fmaf(d1, c[2] + c[3], s_hi[u][0]);
           } else {
             mma(c, a00, a01, a02, a03, qf[1][b][0][0], qf[1][b][0][1]);
             mma(c, a10, a11, a12, a13, qf[1][b][1][0], qf[1][b][1][1]);
 #pragma unroll
             for (int m = 0; m < MINE; ++m) {
-              s_lo[m] = fmaf(d0, c[m], s_lo[m]);
-              s_hi[m] = fmaf(d1, c[2 + m], s_hi[m]);
+              s_lo[u][m] = fmaf(d0, c[m], s_lo[u][m]);
+              s_hi[u][m] = fmaf(d1, c[2 + m], s_hi[u][m]);
             }
           }
         }
-      }
-      __align__(8) uint32_t dv_lo[NB / 2], dv_hi[NB / 2];
-      load_words<NB / 2>(dv_lo, scales + Cfg::kRecord);
-      load_words<NB / 2>(dv_hi, scales + Cfg::kRecord + 8 * (2 * NB));
-#pragma unroll
-      for (int m = 0; m < MINE; ++m) {
-        s_lo[m] *= unscale[m];
-        s_hi[m] *= unscale[m];
-      }
-      if (page < inner0 || page >= inner1) {
-        // a masked token's rows may hold anything: neither its score nor its scales are looked at
-        const int pos_lo = page * kPage + row_lo, pos_hi = pos_lo + 8;
-        const bool live_lo = pos_lo >= run.span.begin && pos_lo < run.span.end, live_hi = pos_hi >= run.span.begin && pos_hi < run.span.end;
+        load_words<NB / 2>(dv_lo[u], scales + u * Cfg::kBoth + Cfg::kRecord);
+        load_words<NB / 2>(dv_hi[u], scales + u * Cfg::kBoth + Cfg::kRecord + 8 * (2 * NB));
 #pragma unroll
         for (int m = 0; m < MINE; ++m) {
-          if (!live_lo) s_lo[m] = -INFINITY;
-          if (!live_hi) s_hi[m] = -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < NB / 2; ++i) {
-          if (!live_lo) dv_lo[i] = 0u;
-          if (!live_hi) dv_hi[i] = 0u;
+          s_lo[u][m] *= unscale[m];
+          s_hi[u][m] *= unscale[m];
         }
       }
-      __half2 largest = __hmax2(__habs2(halves(dv_lo[0])), __habs2(halves(dv_hi[0])));
+      if (page < inner0 || page + PAGES > inner1) {
+        // a masked token's rows may hold anything: neither its score nor its scales are looked at
 #pragma unroll
-      for (int i = 1; i < NB / 2; ++i) largest = __hmax2(largest, __hmax2(__habs2(halves(dv_lo[i])), __habs2(halves(dv_hi[i]))));
-      bool rises = !__hble2(largest, top_half);
+        for (int u = 0; u < PAGES; ++u) {
+          const int pos_lo = (page + u) * kPage + g, pos_hi = pos_lo + 8;
+          const bool live_lo = pos_lo >= run.span.begin && pos_lo < end_of_run, live_hi = pos_hi >= run.span.begin && pos_hi < end_of_run;
 #pragma unroll
-      for (int m = 0; m < MINE; ++m) rises = rises || !(s_lo[m] <= limit[m]) || !(s_hi[m] <= limit[m]);
+          for (int m = 0; m < MINE; ++m) {
+            if (!live_lo) s_lo[u][m] = -INFINITY;
+            if (!live_hi) s_hi[u][m] = -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < NB / 2; ++i) {
+            if (!live_lo) dv_lo[u][i] = 0u;
+            if (!live_hi) dv_hi[u][i] = 0u;
+          }
+        }
+      }
+      __half2 largest = __float2half2_rn(0.0f);
+      bool rises = false;
+#pragma unroll
+      for (int u = 0; u < PAGES; ++u) {
+#pragma unroll
+        for (int i = 0; i < NB / 2; ++i) largest = __hmax2(largest, __hmax2(__habs2(halves(dv_lo[u][i])), __habs2(halves(dv_hi[u][i]))));
+#pragma unroll
+        for (int m = 0; m < MINE; ++m) rises = rises || !(s_lo[u][m] <= limit[m]) || !(s_hi[u][m] <= limit[m]);
+      }
+      rises = rises || !__hble2(largest, top_half);
       if (__any_sync(0xffffffffu, rises)) {
         // an infinite scale spoils its own columns only: the reference stays finite
         float scale = fminf(fmaxf(__low2float(largest), __high2float(largest)), 65504.0f), shrink = 1.0f;
@@ -531,7 +550,9 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
         float f[MINE];
 #pragma unroll
         for (int m = 0; m < MINE; ++m) {
-          float most = fmaxf(s_lo[m], s_hi[m]);
+          float most = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < PAGES; ++u) most = fmaxf(most, fmaxf(s_lo[u][m], s_hi[u][m]));
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
           f[m] = 1.0f;
@@ -549,58 +570,61 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
           o[i][0] *= f[0]; o[i][1] *= f[MINE - 1]; o[i][2] *= f[0]; o[i][3] *= f[MINE - 1];
         }
       }
-      // Weights, and their products with the V scales as value and rest, transposed into operand order. All in f16: w is the weight's value
-      // and x its rest, w * d rounds to the product's value, and fma gives what that leaves out exactly, to which x * d is added.
-      uint32_t pf[PAIRS ? 1 : 2][NB][2];
-      float p_lo[MINE], p_hi[MINE];
 #pragma unroll
-      for (int m = 0; m < MINE; ++m) {
-        p_lo[m] = exp2_flushed(s_lo[m] - sub[m]);
-        p_hi[m] = exp2_flushed(s_hi[m] - sub[m]);
-        weight[m] += p_lo[m] + p_hi[m];
-      }
-      auto product = [](__half2 w, __half2 x, __half2 d, __half2& value, __half2& rest) {
-        value = __hmul2(w, d);
-        rest = __hfma2(x, d, __hfma2(w, d, __hneg2(value)));
-      };
-      auto rest_of = [](float u, float v, __half2 value) { return __floats2half2_rn(u - __low2float(value), v - __high2float(value)); };
-      if constexpr (PAIRS) {
-        const __half2 w = __floats2half2_rn(p_lo[0], p_hi[0]), x = rest_of(p_lo[0], p_hi[0], w);
-        const __half2 w_lo = __low2half2(w), w_hi = __high2half2(w), x_lo = __low2half2(x), x_hi = __high2half2(x);
+      for (int u = 0; u < PAGES; ++u) {
+        // Weights, and their products with the V scales as value and rest, transposed into operand order. All in f16: w is the weight's value
+        // and x its rest, w * d rounds to the product's value, and fma gives what that leaves out exactly, to which x * d is added.
+        uint32_t pf[PAIRS ? 1 : 2][NB][2];
+        float p_lo[MINE], p_hi[MINE];
 #pragma unroll
-        for (int i = 0; i < NB / 2; ++i) {  // two blocks at a time
-          __half2 value_lo, rest_lo, value_hi, rest_hi;
-          product(w_lo, x_lo, __hmul2(halves(dv_lo[i]), to_range), value_lo, rest_lo);
-          product(w_hi, x_hi, __hmul2(halves(dv_hi[i]), to_range), value_hi, rest_hi);
-          pf[0][2 * i][0] = transpose8(bits(__lows2half2(value_lo, rest_lo)));
-          pf[0][2 * i][1] = transpose8(bits(__lows2half2(value_hi, rest_hi)));
-          pf[0][2 * i + 1][0] = transpose8(bits(__highs2half2(value_lo, rest_lo)));
-          pf[0][2 * i + 1][1] = transpose8(bits(__highs2half2(value_hi, rest_hi)));
+        for (int m = 0; m < MINE; ++m) {
+          p_lo[m] = exp2_flushed(s_lo[u][m] - sub[m]);
+          p_hi[m] = exp2_flushed(s_hi[u][m] - sub[m]);
+          weight[m] += p_lo[m] + p_hi[m];
         }
-      } else {
-        const __half2 w_lo = __floats2half2_rn(p_lo[0], p_lo[1]), x_lo = rest_of(p_lo[0], p_lo[1], w_lo);
-        const __half2 w_hi = __floats2half2_rn(p_hi[0], p_hi[1]), x_hi = rest_of(p_hi[0], p_hi[1], w_hi);
+        auto rest_of = [](float v0, float v1, __half2 value) { return __floats2half2_rn(v0 - __low2float(value), v1 - __high2float(value)); };
+        if constexpr (PAIRS) {
+          const __half2 w = __floats2half2_rn(p_lo[0], p_hi[0]), x = rest_of(p_lo[0], p_hi[0], w);
+          const __half2 lo = __lows2half2(w, x), hi = __highs2half2(w, x), to_rest = __floats2half2_rn(0.0f, 1.0f);
+          // (w, x) * d, rounded; what the first product's rounding leaves out is added to the second
+          auto both = [&](__half2 wx, __half2 d) {
+            const __half2 rounded = __hmul2(wx, d);
+            return bits(__hfma2(__low2half2(__hfma2(wx, d, __hneg2(rounded))), to_rest, rounded));
+          };
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {  // two heads at a time
-          const __half2 d_lo = __hmul2(halves(dv_lo[b / 2]), to_range), d_hi = __hmul2(halves(dv_hi[b / 2]), to_range);
-          __half2 value_lo, rest_lo, value_hi, rest_hi;
-          product(w_lo, x_lo, b & 1 ? __high2half2(d_lo) : __low2half2(d_lo), value_lo, rest_lo);
-          product(w_hi, x_hi, b & 1 ? __high2half2(d_hi) : __low2half2(d_hi), value_hi, rest_hi);
-          pf[0][b][0] = transpose8(bits(value_lo));
-          pf[0][b][1] = transpose8(bits(value_hi));
-          pf[1][b][0] = transpose8(bits(rest_lo));
-          pf[1][b][1] = transpose8(bits(rest_hi));
+          for (int i = 0; i < NB / 2; ++i) {
+            const __half2 d_lo = __hmul2(halves(dv_lo[u][i]), to_range), d_hi = __hmul2(halves(dv_hi[u][i]), to_range);
+            pf[0][2 * i][0] = transpose8(both(lo, __low2half2(d_lo)));
+            pf[0][2 * i][1] = transpose8(both(hi, __low2half2(d_hi)));
+            pf[0][2 * i + 1][0] = transpose8(both(lo, __high2half2(d_lo)));
+            pf[0][2 * i + 1][1] = transpose8(both(hi, __high2half2(d_hi)));
+          }
+        } else {
+          auto product = [](__half2 w, __half2 x, __half2 d, __half2& value, __half2& rest) {
+            value = __hmul2(w, d);
+            rest = __hfma2(x, d, __hfma2(w, d, __hneg2(value)));
+          };
+          const __half2 w_lo = __floats2half2_rn(p_lo[0], p_lo[1]), x_lo = rest_of(p_lo[0], p_lo[1], w_lo);
+          const __half2 w_hi = __floats2half2_rn(p_hi[0], p_hi[1]), x_hi = rest_of(p_hi[0], p_hi[1], w_hi);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {  // two heads at a time
+            const __half2 d_lo = __hmul2(halves(dv_lo[u][b / 2]), to_range), d_hi = __hmul2(halves(dv_hi[u][b / 2]), to_range);
+            __half2 value_lo, rest_lo, value_hi, rest_hi;
+            product(w_lo, x_lo, b & 1 ? __high2half2(d_lo) : __low2half2(d_lo), value_lo, rest_lo);
+            product(w_hi, x_hi, b & 1 ? __high2half2(d_hi) : __low2half2(d_hi), value_hi, rest_hi);
+            pf[0][b][0] = transpose8(bits(value_lo));
+            pf[0][b][1] = transpose8(bits(value_hi));
+            pf[1][b][0] = transpose8(bits(rest_lo));
+            pf[1][b][1] = transpose8(bits(rest_hi));
+          }
         }
-      }
-      {
-        __align__(8) uint32_t w[4][NB / 2];  // of tokens t, t + 4, t + 8, t + 12: columns 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-        const unsigned char* v_codes = ring + at + Cfg::kRecord + t * (D / 2) + g * (2 * NB);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) load_words<NB / 2>(w[i], v_codes + 4 * i * (D / 2));
+        __align__(16) uint32_t w[2][NB];  // of tokens 2 t and 2 t + 1, and of those eight further
+        const unsigned char* v_codes = ring + at + u * Cfg::kBoth + Cfg::kRecord + t * D + g * (4 * NB);
+        load_words<NB>(w[0], v_codes);
+        load_words<NB>(w[1], v_codes + 4 * D);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          const unsigned pick = b & 1 ? 0x7632u : 0x5410u;
-          const uint32_t x = __byte_perm(w[0][b / 2], w[1][b / 2], pick), y = __byte_perm(w[2][b / 2], w[3][b / 2], pick), x8 = x >> 8, y8 = y >> 8;
+          const uint32_t x = w[0][b], y = w[1][b], x8 = x >> 8, y8 = y >> 8;
           const uint32_t a00 = widen.get<true>(x), a01 = widen.get<false>(x), a02 = widen.get<true>(y), a03 = widen.get<false>(y);
           const uint32_t a10 = widen.get<true>(x8), a11 = widen.get<false>(x8), a12 = widen.get<true>(y8), a13 = widen.get<false>(y8);
 #pragma unroll
@@ -644,9 +668,9 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
 
   // Units that more than one warp has: a record of a unit that begins in this CTA, or the first of one that began before it, and the records
   // behind it up to the unit's end.
-  const bool mine = lane < 2 * WARPS && records[lane % (2 * WARPS)].valid;
+  const bool mine = lane < 2 * kWarps && records[lane % (2 * kWarps)].valid;
   unsigned left = __ballot_sync(0xffffffffu, mine);
-  const unsigned last = __ballot_sync(0xffffffffu, mine && records[lane % (2 * WARPS)].ends);
+  const unsigned last = __ballot_sync(0xffffffffu, mine && records[lane % (2 * kWarps)].ends);
   Ends mine_of = {};
   while (left) {
     const int k = __ffs(left) - 1, end = __ffs(left & last);  // 0: the unit goes on behind this CTA
@@ -663,17 +687,17 @@ __global__ void __launch_bounds__(WARPS * 32, PAIRS ? 16 / WARPS : 12 / WARPS) a
       mine_of.head0 = first.head0;
       mine_of.heads = first.heads;
     }
-    for (int i = threadIdx.x; i < first.heads * D; i += WARPS * 32) {
+    for (int i = threadIdx.x; i < first.heads * D; i += kWarps * 32) {
       const int h = i / D, d = i - h * D;
-      float ref[WARPS], m = -INFINITY, acc = 0.0f, l = 0.0f;
+      float ref[kWarps], m = -INFINITY, acc = 0.0f, l = 0.0f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
+      for (int w = 0; w < kWarps; ++w) {
         const int r = w == k / 2 ? k : 2 * w;
         ref[w] = members >> r & 1 ? refs[r * Cfg::kHeads + h] : -INFINITY;
         m = fmaxf(m, ref[w]);
       }
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
+      for (int w = 0; w < kWarps; ++w) {
         const int r = w == k / 2 ? k : 2 * w;
         const float f = ref[w] == -INFINITY ? 0.0f : exp2_flushed(ref[w] - m);
         if (members >> r & 1) {
@@ -751,13 +775,13 @@ __global__ void __launch_bounds__(kMergeWarps * 32) attention_q4_merge_kernel(Q4
 // Query heads of a KV head in groups of at most eight: with more the accumulators of a warp do not fit its registers.
 int head_groups(int q_heads, int kv_heads) { return (q_heads / kv_heads + 7) / 8; }
 
-template <int D, bool PAIRS, int WARPS>
+template <int D, bool PAIRS>
 cudaError_t launch_t(const Q4Args& a, unsigned ctas, cudaStream_t stream) {
-  auto kernel = attention_q4_kernel<D, PAIRS, WARPS>;
-  constexpr size_t smem = Q4Cfg<D, PAIRS, WARPS>::kSmem;
+  auto kernel = attention_q4_kernel<D, PAIRS>;
+  constexpr size_t smem = Q4Cfg<D, PAIRS>::kSmem;
   const cudaError_t e = opt_in_shared_memory(kernel, smem);
   if (e != cudaSuccess) return e;
-  return launch_chained(kernel, dim3(ctas), dim3(WARPS * 32), smem, stream, a);
+  return launch_chained(kernel, dim3(ctas), dim3(kWarps * 32), smem, stream, a);
 }
 
 }  // namespace
@@ -771,11 +795,9 @@ Q4Plan plan_attention_q4(int batch, int q_heads, int kv_heads, int head_dim, int
   Q4Plan p;
   const int groups = head_groups(q_heads, kv_heads), heads = (q_heads / kv_heads + groups - 1) / groups;
   const int64_t units = (int64_t)batch * kv_heads * groups;
-  const bool narrow = heads <= 4;
-  const int warps = narrow ? 8 : 4, resident = narrow ? 2 : 3;
   p.direct = max_pages <= kDirectPages;
   // as many CTAs as are resident at once, but two pages for every warp where the tables are short
-  p.ctas = p.direct ? units : std::min<int64_t>((int64_t)resident * sm_count, (units * max_pages + 2 * warps - 1) / (2 * warps));
+  p.ctas = p.direct ? units : std::min<int64_t>((int64_t)kResident * sm_count, (units * max_pages + 2 * kWarps - 1) / (2 * kWarps));
   p.scratch_bytes = p.direct ? 0 : (size_t)p.ctas * (2 * heads * (head_dim + kPartPad) * sizeof(float) + sizeof(Ends));
   return p;
 }
@@ -805,8 +827,8 @@ cudaError_t launch_attention_q4(const PoolView& pool, const float* q, const Lane
   a.op_window = op_window;
   const unsigned ctas = (unsigned)plan.ctas;
   cudaError_t e;
-  if (a.heads <= 4) e = pool.head_dim == 128 ? launch_t<128, true, 8>(a, ctas, stream) : launch_t<64, true, 8>(a, ctas, stream);
-  else e = pool.head_dim == 128 ? launch_t<128, false, 4>(a, ctas, stream) : launch_t<64, false, 4>(a, ctas, stream);
+  if (a.heads <= 4) e = pool.head_dim == 128 ? launch_t<128, true>(a, ctas, stream) : launch_t<64, true>(a, ctas, stream);
+  else e = pool.head_dim == 128 ? launch_t<128, false>(a, ctas, stream) : launch_t<64, false>(a, ctas, stream);
   if (e != cudaSuccess) return e;
   if (launches) ++*launches;
   if (plan.direct) return cudaSuccess;

@@ -82,8 +82,8 @@ __global__ void __launch_bounds__(kThreads) q4_append_kernel(PoolView pool, cons
   }
   if (live) {
     const int pos = info.cursor + token, block = page_rows.divide(pos), page = tables[info.table_offset + block], slot = pos - block * page_rows.value;
-    k_row = q4_row(pool, pool.k, page, head, slot);
-    v_row = q4_row(pool, pool.v, page, head, slot);
+    k_row = q4_row(pool, false, page, head, slot);
+    v_row = q4_row(pool, true, page, head, slot);
   }
   q4_store_block(x, false, k_row, part / 4, nb, live);
   q4_store_block(y, true, v_row, part / 4, nb, live);
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kThreads) q4_rows_kernel(PoolView pool, const 
   Q4Part fetched = {0u, 0.0f};
   if (live) {
     const int page = page_rows.divide((int)number);
-    fetched = q4_fetch(q4_row(pool, which == 0 ? pool.k : pool.v, page, head, (int)number - page * page_rows.value), which != 0, part / 4, nb);
+    fetched = q4_fetch(q4_row(pool, which != 0, page, head, (int)number - page * page_rows.value), which != 0, part / 4, nb);
   }
   float v[8];
   q4_unpack(fetched, which != 0, v);

@@ -5,7 +5,8 @@
 // bytes per block as in a GGUF row, and one contiguous run per page and head (1152 bytes for 16 rows of 128). Codes lie in a row so that
 // a thread of an m16n8k16 product finds its operands side by side (attention_q4.cu). With nb = head_dim / 32 blocks b:
 //   K: words [t][b], t < 4: elements 8 t .. 8 t + 7 of the block; even ones in the low half, odd ones in the high half, ascending
-//   V: half words [g][b], g < 8: elements g, g + 8, g + 16, g + 24 of the block, ascending
+//   V: half words [g][b], g < 8: elements g, g + 8, g + 16, g + 24 of the block, ascending; those of two neighbouring rows alternate (pages
+//      of an odd number of rows: row by row)
 #pragma once
 
 #include <cuda_fp16.h>
@@ -18,21 +19,26 @@ namespace etc {
 
 __host__ __device__ __forceinline__ size_t q4_record_bytes(int block_size, int head_dim) { return (size_t)block_size * (head_dim / 32) * 18; }
 
+// Where a row's codes begin and how far apart its half words are.
 struct Q4Row {
-  uint8_t* codes;
+  uint16_t* codes;
   __half* scales;
+  int stride;
 };
-__device__ __forceinline__ Q4Row q4_row(const PoolView& p, void* slab, int page, int head, int slot) {
-  uint8_t* record = reinterpret_cast<uint8_t*>(slab) + ((size_t)page * p.kv_heads + head) * q4_record_bytes(p.block_size, p.head_dim);
-  return {record + (size_t)slot * (p.head_dim / 2), reinterpret_cast<__half*>(record + (size_t)p.block_size * (p.head_dim / 2)) + (size_t)slot * (p.head_dim / 32)};
+__device__ __forceinline__ Q4Row q4_row(const PoolView& p, bool is_v, int page, int head, int slot) {
+  uint8_t* record = reinterpret_cast<uint8_t*>(is_v ? p.v : p.k) + ((size_t)page * p.kv_heads + head) * q4_record_bytes(p.block_size, p.head_dim);
+  const int row_halves = p.head_dim / 4;
+  const bool paired = is_v && p.block_size % 2 == 0;
+  uint16_t* codes = reinterpret_cast<uint16_t*>(record);
+  return {paired ? codes + (size_t)(slot & ~1) * row_halves + (slot & 1) : codes + (size_t)slot * row_halves,
+          reinterpret_cast<__half*>(codes + (size_t)p.block_size * row_halves) + (size_t)slot * (p.head_dim / 32), paired ? 2 : 1};
 }
 
 // One element, for the paths that are not in a hurry.
 __device__ __forceinline__ float q4_value(const Q4Row& row, bool is_v, int d, int nb) {
   const int b = d >> 5, e = d & 31;
-  const int byte = is_v ? 2 * ((e & 7) * nb + b) + (e >> 4) : 4 * ((e >> 3) * nb + b) + 2 * (e & 1) + ((e >> 2) & 1);
-  const int shift = is_v ? (e & 8) >> 1 : (e & 2) << 1;
-  return __fmul_rn((float)(((row.codes[byte] >> shift) & 15) - 8), __half2float(row.scales[b]));
+  const int half = is_v ? ((e & 7) * nb + b) * row.stride : 2 * ((e >> 3) * nb + b) + (e & 1), shift = is_v ? (e >> 3) * 4 : ((e & 7) >> 1) * 4;
+  return __fmul_rn((float)(((row.codes[half] >> shift) & 15) - 8), __half2float(row.scales[b]));
 }
 
 // Quantizes a block by four neighbouring lanes, lane t of which (the lowest two bits) holds elements 8 t .. 8 t + 7, and stores it where
@@ -76,13 +82,12 @@ __device__ __forceinline__ void q4_store_block(const float (&v)[8], bool is_v, c
     };
     const uint32_t even = nibbles(bytes), odd = nibbles(bytes >> 4);
     if (live) {
-      uint16_t* dst = reinterpret_cast<uint16_t*>(row.codes);
-      dst[2 * t * nb + b] = (uint16_t)even;
-      dst[(2 * t + 1) * nb + b] = (uint16_t)odd;
+      row.codes[(2 * t * nb + b) * row.stride] = (uint16_t)even;
+      row.codes[((2 * t + 1) * nb + b) * row.stride] = (uint16_t)odd;
     }
   } else if (live) {
     const uint32_t word = pack([](int i) { return 4 * (i >> 1) + 16 * (i & 1); });
-    uint16_t* dst = reinterpret_cast<uint16_t*>(row.codes) + 2 * (t * nb + b);
+    uint16_t* dst = row.codes + 2 * (t * nb + b);
     if ((reinterpret_cast<uintptr_t>(dst) & 3) == 0) {
       *reinterpret_cast<uint32_t*>(dst) = word;
     } else {  // pages of an odd number of blocks
@@ -100,9 +105,8 @@ struct Q4Part {
 };
 __device__ __forceinline__ Q4Part q4_fetch(const Q4Row& row, bool is_v, int b, int nb) {
   const int t = threadIdx.x & 3;
-  const uint16_t* src = reinterpret_cast<const uint16_t*>(row.codes);
-  const int at = is_v ? 2 * t * nb + b : 2 * (t * nb + b), next = is_v ? at + nb : at + 1;
-  return {src[at] | (uint32_t)src[next] << 16, __half2float(row.scales[b])};
+  const int at = is_v ? (2 * t * nb + b) * row.stride : 2 * (t * nb + b), next = is_v ? at + nb * row.stride : at + 1;
+  return {row.codes[at] | (uint32_t)row.codes[next] << 16, __half2float(row.scales[b])};
 }
 __device__ __forceinline__ void q4_unpack(const Q4Part& part, bool is_v, float (&v)[8]) {
   const int t = threadIdx.x & 3;
