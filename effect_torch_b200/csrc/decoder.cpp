@@ -590,7 +590,7 @@ etc_status enqueue_score(StepContext& s, int active, const ScoreRequest& request
   ETC_TRY(enqueue_layers(s, pending));
   auto score = [&](const float* logits, int64_t row0, int64_t n) -> etc_status {
     ETC_CUDA(launch_logprobs(logits, n, c.vocab, c.vocab, buffers.targets + row0, buffers.logprobs + row0, buffers.entropy + row0, request.top,
-                             buffers.top_tokens + row0 * request.top, buffers.top_logprobs + row0 * request.top, d->rt->d_status, d->rt->sm_count, stream));
+                             buffers.top_tokens + row0 * request.top, buffers.top_logprobs + row0 * request.top, d->rt->d_status, d->rt->sm_count, stream, row0));
     ++s.launches;
     return ETC_OK;
   };

@@ -220,7 +220,7 @@ constexpr int kMaxAlternatives = 32;
 etc_status validate_logprobs(int64_t vocab, int top);  // ops.cpp
 cudaError_t launch_logprobs(const float* logits, int64_t rows, int64_t vocab, int64_t row_stride, const uint32_t* targets, float* logprobs,
                             float* entropy, int top, uint32_t* top_tokens, float* top_logprobs, DeviceStatus* status, int sm_count,
-                            cudaStream_t stream);
+                            cudaStream_t stream, int64_t first_row = 0);  // first_row: what reports count rows from
 cudaError_t launch_embedding_f32(const void* indexes, int index_is_i64, int64_t count, const float* table, int64_t rows,
                                  int64_t columns, float* out, DeviceStatus* status, cudaStream_t stream);
 // Copy row (advance-1) of each lane's [T, width] block into [lanes, width] (LastTokenRow).

@@ -46,6 +46,7 @@ struct LogprobArgs {
   float* top_logprobs;
   DeviceStatus* status;
   int chunks;  // 16-byte pieces of a row per CTA
+  int64_t first_row;
 };
 
 // Larger value -> larger key; of equal values (0 and -0 are equal) the lower token has the larger key. 0 is below every key.
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(Logpr
         }
         if (bad != kNone && atomicCAS(&a.status->code, kStatusNone, kStatusBadLogprobLogit) == kStatusNone) {
           a.status->value = bad;
-          a.status->bound = row;
+          a.status->bound = a.first_row + row;
         }
       }
     }
@@ -384,9 +385,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(Logpr
 
 cudaError_t launch_logprobs(const float* logits, int64_t rows, int64_t vocab, int64_t row_stride, const uint32_t* targets, float* logprobs,
                             float* entropy, int top, uint32_t* top_tokens, float* top_logprobs, DeviceStatus* status, int sm_count,
-                            cudaStream_t stream) {
+                            cudaStream_t stream, int64_t first_row) {
   if (rows == 0) return cudaSuccess;
-  LogprobArgs a = {logits, vocab, row_stride, targets, logprobs, entropy, top, top_tokens, top_logprobs, status, 0};
+  LogprobArgs a = {logits, vocab, row_stride, targets, logprobs, entropy, top, top_tokens, top_logprobs, status, 0, first_row};
   // CTAs per row: what fills the SMs (two CTAs each) in the fewest turns, a turn being a slice at the copy bandwidth and a fixed part.
   const int64_t pieces = (vocab + 3 + 3) / 4;
   unsigned ranks = 1;

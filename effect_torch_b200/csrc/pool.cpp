@@ -247,6 +247,9 @@ etc_status etc_pool_create(etc_runtime* rt, int layers, int kv_heads, int head_d
                                           " must be a positive multiple of block size " + std::to_string(block_size));
   if (dtype == ETC_KV_Q4 && head_dim % 32 != 0)
     return fail(ETC_INVALID_ARGUMENT, "kv pool: the q4 tier needs a head dim that is a multiple of 32, got " + std::to_string(head_dim));
+  if (dtype == ETC_KV_Q4 && (int64_t)max_tokens * kv_heads > INT32_MAX)  // rows of a head are counted in 32 bits
+    return fail(ETC_INVALID_ARGUMENT, "kv pool: the q4 tier holds at most 2^31 - 1 rows of a head, got " + std::to_string(max_tokens) + " tokens of " +
+                                          std::to_string(kv_heads) + " heads");
   etc_pool* p = new etc_pool();
   static std::atomic<uint64_t> next_uid{1};
   p->uid = next_uid.fetch_add(1);

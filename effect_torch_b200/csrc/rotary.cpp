@@ -58,6 +58,7 @@ etc_status rope_frequencies(const etc_rope_config& c, const float* divisors, std
       const double stretched = std::min(1.0, std::max(0.0, ((double)j - low) / std::max(high - low, 0.001)));
       f = f / c.factor * stretched + f * (1.0 - stretched);
     }
+    if (!std::isfinite(f)) return bad("the frequency of pair " + std::to_string(j) + " is not finite");
     (*inv_freq)[(size_t)j] = f;
   }
   *magnitude = c.attention_factor > 0.0 ? c.attention_factor : c.scaling == ETC_ROPE_SCALING_YARN ? 0.1 * std::log(c.factor) + 1.0 : 1.0;

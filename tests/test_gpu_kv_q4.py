@@ -381,3 +381,8 @@ def test_what_is_refused():
             rt.synchronize()
         assert not rows.cpu().numpy().any()
     rt.synchronize()
+
+
+def test_more_rows_than_32_bits_count_are_refused():
+    with pytest.raises(et.BackendError, match="at most 2\\^31 - 1 rows"):  # before anything is allocated
+        et.NativeKvPool(runtime(), 1, 32, 32, 1 << 26, 16, et.KV_Q4)

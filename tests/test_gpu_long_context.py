@@ -3,6 +3,8 @@
 The plain model attends over the rows that the decoder's cache holds (read back), after checking that each is what its own key or value
 row is kept as, give or take a step of its block: a row whose f32 or f16 rounding differs may take the neighbouring code, and both are right.
 Logits are held to what the decoder is held to elsewhere: 1e-5 (reference-order f32) and 2e-3 (f16 activations) of the largest."""
+import re
+
 import numpy as np
 import pytest
 
@@ -215,6 +217,22 @@ def test_more_rows_than_logits_exist_at_a_time():
     w = helpers.make_weights(cfg, seed=7, codec=orc.Q4_0)
     dec, pool, plain = make(cfg, w, 5, et.KV_F16, False, None, max_tokens=640, max_advance=64)
     run(dec, pool, plain, et.KV_F16, 2e-3, (64, 64), 5, scored=True)  # 320 rows: 256 and 64
+
+
+def test_a_bad_logit_is_reported_with_its_row():
+    """Row of the step (lane 4's are 256 to 319), not of the 256 rows whose logits exist at a time. In f32: activations in f16 are held to
+    finite numbers, so that a NaN does not reach their logits."""
+    cfg = dict(SMALL, layers=1)
+    w = helpers.make_weights(cfg, seed=7)
+    w["tok_embd"][77] = np.nan
+    dec, pool, _ = make(cfg, w, 5, et.KV_F32, True, None, max_tokens=640, max_advance=64)
+    tokens = np.random.default_rng(1).integers(0, 77, (5, 64)).astype(np.uint32)
+    tokens[4, 60] = 77
+    seqs = [pool.makeSequence() for _ in range(5)]
+    with pytest.raises(et.BackendError, match="logit") as e:
+        dec.score(pool, seqs, tokens, tokens)
+    assert 256 <= int(re.search(r"of row (\d+) is NaN", str(e.value)).group(1)) < 320
+    assert [s.cursor for s in seqs] == [0] * 5
 
 
 def test_a_step_that_fails_changes_nothing():

@@ -81,6 +81,12 @@ def test_refusals(change, message):
     assert e.value.reason == "compilation-failed"
 
 
+def test_frequencies_beyond_f64_are_refused():
+    """1e-300^(-62/64) / 1e-38 is some 1e328."""
+    with pytest.raises(et.BackendError, match="frequency of pair 31 is not finite"):
+        et.rope_frequencies(et.rope_config(64, theta=1e-300), [1.0] * 31 + [1e-38])
+
+
 def test_rust_mirrors_the_config():
     header = open(os.path.join(ROOT, "include", "et_cuda.h")).read()
     body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct etc_rope_config \{(.*?)\} etc_rope_config;", header, flags=re.S).group(1), flags=re.S)
