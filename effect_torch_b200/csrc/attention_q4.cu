@@ -525,19 +525,24 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
           }
         }
       }
-      __half2 largest = __float2half2_rn(0.0f);
-      bool rises = false;
+      auto largest_scale = [&](auto&& of) {
+        __half2 largest = __float2half2_rn(0.0f);
 #pragma unroll
-      for (int u = 0; u < PAGES; ++u) {
+        for (int u = 0; u < PAGES; ++u)
 #pragma unroll
-        for (int i = 0; i < NB / 2; ++i) largest = __hmax2(largest, __hmax2(__habs2(halves(dv_lo[u][i])), __habs2(halves(dv_hi[u][i]))));
+          for (int i = 0; i < NB / 2; ++i) largest = __hmax2(largest, __hmax2(of(__habs2(halves(dv_lo[u][i]))), of(__habs2(halves(dv_hi[u][i])))));
+        return largest;
+      };
+      __half2 largest = largest_scale([](__half2 d) { return d; });
+      bool rises = !__hble2(largest, top_half);
+#pragma unroll
+      for (int u = 0; u < PAGES; ++u)
 #pragma unroll
         for (int m = 0; m < MINE; ++m) rises = rises || !(s_lo[u][m] <= limit[m]) || !(s_hi[u][m] <= limit[m]);
-      }
-      rises = rises || !__hble2(largest, top_half);
       if (__any_sync(0xffffffffu, rises)) {
-        // an infinite scale spoils its own columns only: the reference stays finite
-        float scale = fminf(fmaxf(__low2float(largest), __high2float(largest)), 65504.0f), shrink = 1.0f;
+        // an infinite scale spoils the columns of its block, and nothing else: infinity times 0 takes no part in a maximum
+        largest = largest_scale([](__half2 d) { return __hmul2(d, __hle2(d, __float2half2_rn(65504.0f))); });
+        float scale = fmaxf(__low2float(largest), __high2float(largest)), shrink = 1.0f;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) scale = fmaxf(scale, __shfl_xor_sync(0xffffffffu, scale, off));
         if (scale > top_scale) {

@@ -386,3 +386,21 @@ def test_what_is_refused():
 def test_more_rows_than_32_bits_count_are_refused():
     with pytest.raises(et.BackendError, match="at most 2\\^31 - 1 rows"):  # before anything is allocated
         et.NativeKvPool(runtime(), 1, 32, 32, 1 << 26, 16, et.KV_Q4)
+
+
+@pytest.mark.parametrize("q_heads", [4, 8])
+@pytest.mark.parametrize("length", [20, 900])
+def test_an_infinite_scale_spoils_its_block_only(q_heads, length):
+    """One value beyond the scales' range: the columns of its block have no result, those of the others are as precise as without it."""
+    D = 128
+    cache = Cache([length], 1, D, seed=5)
+    q = np.random.default_rng(7).normal(size=(1, q_heads, D)).astype(np.float32)
+    lanes, pages = [(length - 1, 1, 0, cache.first[0])], -(-length // PAGE)
+    want, room = expected(cache, q, 0.1, lanes)
+    v = cache.v[0].copy()
+    v[0, length // 2, 70] = 1e6
+    runtime().paged_append_into(cache.pool, 0, lanes_of([[0, length, 0, cache.first[0]]]), cache.tables, 1, length, dev(cache.k[0][None]), dev(v[None]))
+    got = attend(cache, q, 0.1, lanes, pages)
+    others = np.r_[0:64, 96:128]
+    assert not np.isfinite(got[..., 64:96]).any()
+    check(got[..., others], want[..., others], room[..., others])
