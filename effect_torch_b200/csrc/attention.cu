@@ -1,4 +1,4 @@
-// Paged KV kernels for sm_100a: page-pool append (all four tiers), reference-order attention in
+// Paged KV kernels for sm_100a: page-pool append (all tiers), reference-order attention in
 // f64, tensor-core flash-decoding over the block table with split-KV merge, RoPE and append inside
 // both for a decoder's one-token steps, and as a kernel of their own for chunks.
 //
@@ -9,7 +9,9 @@
 // HBM layout (chosen for the B200, not the reference's token-major slab): per layer one K and
 // one V slab of [pages][kv_heads][block_size][head_dim] elements, so the block_size rows of one
 // (page, head) are one contiguous run (4 KiB for f16, 16 tokens, D=128) that a warp fetches
-// with 16-byte cp.async copies. u8 tier scales are [pages][kv_heads][block_size] f32.
+// with 16-byte cp.async copies. u8 tier scales are [pages][kv_heads][block_size] f32. The 4-bit
+// tier's pages are records of codes and scales (kv_q4.cuh); its decode attention is a kernel of its
+// own (attention_q4.cu), its chunks are widened to f16 tiles here.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

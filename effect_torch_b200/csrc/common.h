@@ -37,9 +37,9 @@ etc_status fail(etc_status status, const std::string& message);
 // Device-side status word. Kernels record the first problem they see with one atomicCAS on
 // `code`; the host reads it at synchronising calls and turns it into ETC_EXECUTION.
 struct DeviceStatus {
-  unsigned long long code;     // 0 none, 1 embedding index out of range, 2 non-finite logit
-  long long value;             // offending index / token position
-  long long bound;             // rows / vocabulary
+  unsigned long long code;     // 0 none, or what was found first (below; 3 and 4: a wait that ran out)
+  long long value;             // offending index / token position / row / target
+  long long bound;             // rows / vocabulary / the row that the value is in
   long long reserved;
 };
 enum : unsigned long long {

@@ -1,6 +1,7 @@
 // Rows into and out of pages held in 4 bits (kv_q4.cuh). Four neighbouring threads to a block of 32 values, eight each: loads and stores
-// of values are 32 bytes per thread and whole lines per warp, codes are put in their places by shuffles among the four. Bound by
-// HBM on the f32 side (4 bytes a value against 0.56).
+// of values are 32 bytes per thread and whole lines per warp, codes are put in their places by shuffles among the four. The bytes
+// are f32 ones (4 a value against 0.56), but large appends are bound by instructions, some 24 per value (extreme of the block, code,
+// packing): 8 lanes of 509 tokens, 8 heads of 128, in and out in 21.6 us (76 MB, 3530 GB/s); calls of one token by their launches.
 #include <algorithm>
 #include <initializer_list>
 

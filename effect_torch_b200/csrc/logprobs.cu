@@ -11,6 +11,9 @@
 // looks at each such thread's values again (some hundred, from L2), lists those that reach the bound, and the list is ranked by
 // counting. Should the list overflow (an order of logits made for it), the alternatives are found one after the other instead.
 //
+// Bound by HBM where rows are many, 2048 of 128256 (1.05 GB) 169 to 176 us = 6.0 to 6.2 TB/s of a copy's 6.55; by latency where they are
+// few, one with 20 alternatives 10.7 us, 32 with 5 alternatives 11.5.
+//
 // Sums are f32 within a thread (some 250 values of a long vocabulary) and a warp, f64 from the warps on.
 #include <cooperative_groups.h>
 

@@ -4,7 +4,8 @@
 //
 // for the pairs (a, b) = (j, R/2 + j) or (2j, 2j + 1) of the first R values of a head; the others are copied.
 //
-// Bound by HBM once a launch is large: a value is read and written once, 8 bytes. What stands in the way of that is the angle of far
+// Bound by HBM once a launch is large: a value is read and written once, 8 bytes; 4096 positions of 72 heads of 128 (302 MB) take 53.7 us =
+// 5630 GB/s (a copy: 6555), a decode step of 32 positions is a launch, 3.5 us. What stands in the way of that is the angle of far
 // positions, which f32 does not hold: position * f_j is taken in f64, in half turns (the table holds f_j / pi), reduced there
 // to [-1, 1] by whole turns, and only the rest goes through the f32 sine and cosine, its own rounding added back to first order. That
 // is six f64 instructions per angle where a sine and cosine in f64 are some hundred. A thread keeps four neighbouring pairs and

@@ -155,6 +155,7 @@ fn kv_dtype(name: &str) -> Result<i32> {
         "f16" => Ok(ffi::ETC_KV_F16),
         "bf16" => Ok(ffi::ETC_KV_BF16),
         "u8" => Ok(ffi::ETC_KV_U8),
+        "q4" => Ok(ffi::ETC_KV_Q4),
         other => Err(Error::new(Status::InvalidArg, format!("kv state: dtype {other} is not a KV tier"))),
     }
 }

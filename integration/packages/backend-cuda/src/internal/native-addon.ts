@@ -78,7 +78,7 @@ export declare class Executable {
 }
 
 /** KV tiers of the pool. @internal */
-export type NativeDType = "f32" | "f16" | "bf16" | "u8"
+export type NativeDType = "f32" | "f16" | "bf16" | "u8" | "q4"
 /** Native spelling of the two supported rotary coordinate layouts. @internal */
 export type NativeRotaryLayout = "HalfSplit" | "InterleavedPairs"
 /** Tensor formats the decode path reads. @internal */
