@@ -56,9 +56,10 @@ constexpr float kSmallestScale = 5.9604645e-8f;  // 2^-24, the smallest f16
 // What a CTA has of units that other CTAs have parts of: the end of one that began before it (part 0), the beginning of one that goes on
 // behind it (part 1).
 struct Ends {
-  int open, open_ends;  // there is a part 0; the unit ends in it
+  int open;             // there is a part 0
   int tail;             // there is a part 1, of:
   int row, head0, heads;
+  int last;             // the CTA in which that unit ends
   int unused[2];
 };
 
@@ -241,6 +242,7 @@ __device__ __forceinline__ void load_words(uint32_t* dst, const unsigned char* s
 struct Record {
   int valid, ends;     // ends: the unit's last page is in it
   int row, head0, heads;
+  long long end;       // the place where the unit ends
 };
 
 // A warp's run of work: the unit it is in and its pages there.
@@ -295,6 +297,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
       if (span_of(a.lanes[l], a.op_window).pages == 0)
         for (int i = threadIdx.x; i < a.q_heads * D; i += kWarps * 32) store_out(a, D, l, i, 0.0f);
   }
+  __shared__ long long total_places;
   __shared__ Record records[2 * kWarps];  // of each warp the unit that began before its run, the unit that goes on behind it
   if (lane < 2) records[2 * warp + lane].valid = 0;
   bool works = true;
@@ -314,6 +317,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
     clip(run, kUnitPages + from);
   } else {
     const long long total = all_places(a) * units;
+    if (threadIdx.x == 0) total_places = total;
     const int runs = (int)gridDim.x * kWarps, mine = (int)blockIdx.x * kWarps + warp;
     const long long begin = total * mine / runs;
     run.stop = total * (mine + 1) / runs;
@@ -649,7 +653,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
     const float back = 1.0f / __low2float(to_range);  // the weights' own 2^kWeightBits cancels against that of their sum
     const bool begins = run.page0 == run.span.first, ends = run.page1 == run.span.first + run.span.pages;
     const int record = 2 * warp + (begins ? 1 : 0);
-    if (lane == 0 && !(begins && ends)) records[record] = Record{1, ends, run.lane, head0, live_heads};
+    if (lane == 0 && !(begins && ends)) records[record] = Record{1, ends, run.lane, head0, live_heads, run.stop + (run.span.first + run.span.pages - run.page1)};
 #pragma unroll
     for (int m = 0; m < MINE; ++m) {
 #pragma unroll
@@ -687,12 +691,14 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
     const Record first = records[k];
     if (open) {
       mine_of.open = 1;
-      mine_of.open_ends = end != 0;
     } else if (!end) {
       mine_of.tail = 1;
       mine_of.row = first.row;
       mine_of.head0 = first.head0;
       mine_of.heads = first.heads;
+      // a run holds the places from total * run / runs on
+      const long long place = records[31 - __clz(members)].end - 1;
+      mine_of.last = (int)(((place + 1) * ((int)gridDim.x * kWarps) - 1) / total_places) / kWarps;
     }
     for (int i = threadIdx.x; i < first.heads * D; i += kWarps * 32) {
       const int h = i / D, d = i - h * D;
@@ -725,12 +731,12 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
 }
 
 // Adds up the parts of units that were cut: grid (heads of a unit, CTAs of the attention kernel), a CTA for the unit that goes on behind
-// its namesake, if there is one. Latency-bound: eight warps take the parts in turn, a thread D / 32 columns of them; a reference is
-// fetched with its part. (One CTA per unit, a part after the other: 150 of 182 us for one lane in 37 parts; a CTA for every unit and
+// its namesake, if there is one. Latency-bound: four warps take the parts in turn, four at a time, a thread D / 32 columns of them; a
+// reference is fetched with its part. (One CTA per unit, a part after the other: 150 of 182 us for one lane in 37 parts; a CTA for every unit and
 // head, which worked out by 64-bit divisions whether its unit was cut: 14 us for 64 lanes.)
-constexpr int kMergeWarps = 8;
+constexpr int kMergeWarps = 4, kMergeParts = 4;
 template <int D>
-__global__ void __launch_bounds__(kMergeWarps * 32) attention_q4_merge_kernel(Q4Args a, int ctas) {
+__global__ void __launch_bounds__(kMergeWarps * 32) attention_q4_merge_kernel(Q4Args a) {
   __shared__ __align__(16) float sums[kMergeWarps][D];
   __shared__ float refs[kMergeWarps], weights[kMergeWarps];
   constexpr int COLUMNS = D / 32;  // of a thread
@@ -739,28 +745,29 @@ __global__ void __launch_bounds__(kMergeWarps * 32) attention_q4_merge_kernel(Q4
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.x, c0 = blockIdx.y;
   const Ends own = a.ends[c0];
   if (!own.tail || h >= own.heads) return;
-  int c1 = c0;  // the CTA in which the unit ends: the first behind c0 whose open unit does
-  for (int from = c0 + 1; from < ctas; from += 32) {
-    const int c = from + lane;
-    const unsigned found = __ballot_sync(0xffffffffu, c < ctas && a.ends[c].open_ends);
-    if (found) {
-      c1 = from + __ffs(found) - 1;
-      break;
-    }
-  }
   float m = -INFINITY, l = 0.0f, acc[COLUMNS] = {};
-  for (int c = c0 + warp; c <= c1; c += kMergeWarps) {
-    if (c > c0 && !a.ends[c].open) continue;  // more CTAs than places: it has none
-    const float* part = a.partial + ((size_t)(2 * c + (c == c0 ? 1 : 0)) * a.heads + h) * (D + kPartPad);
-    float x[COLUMNS];
+  for (int first = c0 + warp; first <= own.last; first += kMergeWarps * kMergeParts) {
+    float x[kMergeParts][COLUMNS], r[kMergeParts], w[kMergeParts];
+    bool there[kMergeParts];  // with more CTAs than places some have no part
 #pragma unroll
-    for (int j = 0; j < COLUMNS; ++j) x[j] = part[lane + 32 * j];
-    const float r = part[D], w = part[D + 1], to = fmaxf(m, r);
-    const float old = m == -INFINITY ? 0.0f : exp2_flushed(m - to), f = r == -INFINITY ? 0.0f : exp2_flushed(r - to);
-    m = to;
-    l = l * old + w * f;
+    for (int u = 0; u < kMergeParts; ++u) {
+      const int c = min(first + u * kMergeWarps, own.last);
+      const float* part = a.partial + ((size_t)(2 * c + (c == c0 ? 1 : 0)) * a.heads + h) * (D + kPartPad);
 #pragma unroll
-    for (int j = 0; j < COLUMNS; ++j) acc[j] = acc[j] * old + x[j] * f;
+      for (int j = 0; j < COLUMNS; ++j) x[u][j] = part[lane + 32 * j];
+      r[u] = part[D];
+      w[u] = part[D + 1];
+      there[u] = first + u * kMergeWarps <= own.last && (c == c0 || a.ends[c].open);
+    }
+#pragma unroll
+    for (int u = 0; u < kMergeParts; ++u) {
+      if (!there[u]) continue;
+      const float to = fmaxf(m, r[u]), old = m == -INFINITY ? 0.0f : exp2_flushed(m - to), f = r[u] == -INFINITY ? 0.0f : exp2_flushed(r[u] - to);
+      m = to;
+      l = l * old + w[u] * f;
+#pragma unroll
+      for (int j = 0; j < COLUMNS; ++j) acc[j] = acc[j] * old + x[u][j] * f;
+    }
   }
 #pragma unroll
   for (int j = 0; j < COLUMNS; ++j) sums[warp][lane + 32 * j] = acc[j];
@@ -840,7 +847,7 @@ cudaError_t launch_attention_q4(const PoolView& pool, const float* q, const Lane
   if (launches) ++*launches;
   if (plan.direct) return cudaSuccess;
   e = launch_chained(pool.head_dim == 128 ? attention_q4_merge_kernel<128> : attention_q4_merge_kernel<64>, dim3((unsigned)a.heads, ctas), dim3(kMergeWarps * 32), 0,
-                     stream, a, (int)plan.ctas);
+                     stream, a);
   if (e == cudaSuccess && launches) ++*launches;
   return e;
 }
