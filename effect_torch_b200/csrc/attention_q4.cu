@@ -15,8 +15,8 @@
 // adds the two sums of its head; five to eight as they are, with a second product for the rests onto the same sums.
 //
 // What bounds it is instructions and their latency, not HBM: some 350 per page and warp, 152 of them widening codes, at 2.3 per cycle of an
-// SM with 12 warps. 64 lanes of 128 to 4096 tokens (32 query heads, 8 KV heads of 128; 158 MB) 46.3 us = 3400 GB/s, one of 131072
-// 45.0 us = 3360, 16 lanes of 1024 to 16384 with 64 heads 60.1 us = 2690 (the copy bandwidth is 6555).
+// SM with 12 warps. 64 lanes of 128 to 4096 tokens (32 query heads, 8 KV heads of 128; 158 MB) 45.6 us = 3470 GB/s, one of 131072
+// 43.5 us = 3470, 16 lanes of 1024 to 16384 with 64 heads 59.5 us = 2710 (the copy bandwidth is 6555).
 //
 // Work. The pages of all (lane, KV head) units in a row are cut into as many equal runs as there are warps, whatever the lengths of the
 // lanes: nobody waits for the longest. A warp takes its run by pages, or pairs of them, through a ring of cp.async copies that runs on

@@ -65,6 +65,20 @@ def test_sizes(batch, heads, steps):
     check(host(out), *expected(x, offsets, table))
 
 
+@pytest.mark.parametrize("layout", [et.HALF_SPLIT, et.INTERLEAVED_PAIRS])
+@pytest.mark.parametrize("head_dim,rotary", [(64, 64), (64, 20), (32, 6), (128, 128), (20, 4)])
+@pytest.mark.parametrize("batch,heads,steps", [(9001, 1, 1), (3100, 3, 3), (1, 5, 9473), (140, 2, 67), (401, 7, 23), (600, 1, 16)])
+def test_several_positions_at_a_time(batch, heads, steps, head_dim, rotary, layout):
+    """Many positions of few heads, where a group of positions reaches over one, several or many batch entries."""
+    rng = np.random.default_rng(batch + head_dim)
+    table = et.RotaryTable(runtime(), head_dim, rotary_dim=rotary, layout=layout, **RULES[2])
+    x = rng.normal(size=(batch, heads, steps, head_dim)).astype(np.float32)
+    offsets = rng.integers(0, 1 << 17, batch)
+    out = empty(x.shape)
+    runtime().rotary_into(table, dev(x), dev(offsets), batch, heads, steps, out)
+    check(host(out), *expected(x, offsets, table))
+
+
 @pytest.mark.parametrize("start", [0, 1, 4])
 def test_heads_inside_the_rows_of_a_fused_projection(start):
     """q and k heads of [batch, steps, q + 2 kv, D] rows, where the rows start anywhere; v and what lies around stay."""
