@@ -11,7 +11,7 @@
 // looks at each such thread's values again (some hundred, from L2), lists those that reach the bound, and the list is ranked by
 // counting. Should the list overflow (an order of logits made for it), the alternatives are found one after the other instead.
 //
-// Bound by HBM where rows are many, 2048 of 128256 (1.05 GB) 169 to 176 us = 6.0 to 6.2 TB/s of a copy's 6.55; by latency where they are
+// Bound by HBM where rows are many, 2048 of 128256 (1.05 GB) 163.5 us = 6.4 TB/s of a copy's 6.55; by latency where they are
 // few, one with 20 alternatives 10.7 us, 32 with 5 alternatives 11.5.
 //
 // Sums are f32 within a thread (some 250 values of a long vocabulary) and a warp, f64 from the warps on.
@@ -204,9 +204,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(Logpr
       for (int u = 0; u < kBatch; ++u) v[u] = load(p + (int64_t)u * kThreads);
       take(v, p, kBatch);
     }
-    for (; p < piece1; p += kThreads) {
-      v[0] = load(p);
-      take(v, p, 1);
+    if constexpr (TOP) {
+      for (; p < piece1; p += kThreads) {
+        v[0] = load(p);
+        take(v, p, 1);
+      }
+    } else if (p < piece1) {  // at once, too (with alternatives that needs more than it saves: 344 us against 232 for 2048 rows of 128256)
+      const int n = (int)((piece1 - p + kThreads - 1) / kThreads);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (u < n) v[u] = load(p + (int64_t)u * kThreads);
+      take(v, p, n);
     }
   }
 
@@ -391,18 +399,13 @@ cudaError_t launch_logprobs(const float* logits, int64_t rows, int64_t vocab, in
                             cudaStream_t stream, int64_t first_row) {
   if (rows == 0) return cudaSuccess;
   LogprobArgs a = {logits, vocab, row_stride, targets, logprobs, entropy, top, top_tokens, top_logprobs, status, 0, first_row};
-  // CTAs per row: what fills the SMs (two CTAs each) in the fewest turns, a turn being a slice at the copy bandwidth and a fixed part.
+  // CTAs per row: as many as fill the SMs, two on each, as long as there is a piece for every thread. More rows take one, four of which an SM
+  // holds (400 rows of 128256: 41.1 us against 44.5 by two; 1024: 84.3 against 102.5), but up to two for every SM, which would leave it
+  // half empty, two where rows are long (256 rows of 128256: 30.3 us by two, 38.5 by one, 36.9 by four; of 32000 12.3 and 11.8).
   const int64_t pieces = (vocab + 3 + 3) / 4;
   unsigned ranks = 1;
-  double shortest = 0.0;
-  for (unsigned r = 1; r <= (unsigned)kMaxCluster; r *= 2) {
-    const double turns = (double)((rows * r + 2 * sm_count - 1) / (2 * sm_count));
-    const double time = turns * ((double)((pieces + r - 1) / r) + 1024.0);
-    if (r == 1 || time < shortest) {
-      shortest = time;
-      ranks = r;
-    }
-  }
+  while (ranks < (unsigned)kMaxCluster && rows * ranks <= sm_count && pieces >= 2 * ranks * 512) ranks *= 2;
+  if (rows > sm_count && rows <= 2 * sm_count && pieces >= 16384) ranks = 2;
   a.chunks = (int)((pieces + ranks - 1) / ranks);
   const dim3 grid((unsigned)(rows * ranks));
   auto launch = [&](auto kernel, int threads) { return launch_chained_cluster(kernel, grid, dim3((unsigned)threads), 0, stream, ranks, a); };
