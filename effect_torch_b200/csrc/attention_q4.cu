@@ -1,12 +1,18 @@
-// Decode attention over pages held in 4 bits (kv_q4.cuh): one query token per lane, 16-token pages, head dim 64 or 128, and results as
-// close to the stored values as f32 arithmetic comes.
+// Decode attention over pages held in 4 bits (kv_q4.cuh): one query token per lane, 16-token pages, head dim 64 or 128.
 //
 // Mathematics. With codes c (whole numbers -8 .. 7) and a scale per row and block of 32 columns,
 //   s[tok] = scale * sum_b dk[tok][b] * (sum_{d in b} q[d] ck[tok][d])      o[d] = sum_tok p[tok] dv[tok][b(d)] cv[tok][d] / sum_tok p[tok]
 // so codes go through mma.sync.m16n8k16 as exact f16 numbers, a block of columns at a time, and scales are applied in f32: to the
-// sums of a block (K), to the weights ahead of the product (V). What f16 would round, q and p * dv, is split in two f16 numbers, value and rest
-// (22 bits together), after scaling by powers of two that keep the rest out of the subnormals; the products of both are added in f32.
-// Nothing else is below f32.
+// sums of a block (K), to the weights ahead of the product (V). What f16 would round, q and p * dv, is split in two f16 numbers, value and
+// rest, 22 bits together, and the products of both are added in f32. Scores, weights, their sum and p * dv are f32.
+//
+// What the split costs. A query is scaled by a power of two, its largest value to 2^13 .. 2^14, and its values are held to 2^-22 of themselves or
+// 2^-38 of the largest. For p * dv the power of two is that of the softmax: a head's reference is the largest (score + log2 of the token's
+// largest |dv|), not the largest score, so that the largest product is 2^11 or more whatever the scales are. Products are held to 2^-22 of themselves, or to
+// half of the smallest f16 number, 2^-36 of the largest one: a token whose weight is next to nothing adds that error once. With up to four heads
+// (below) rests have columns and sums of their own and are held times 2^11, which makes it 2^-47. (A reference of scores alone and one power of
+// two for all dv of a run were 2.3 us faster over 64 lanes, and off by 3 % in a block whose scales are 1e6 below another's, and by
+// 3e-6 to 5e-5 where one token draws most of the weight of 131072.) What remains is the tensor core's own sums, 16 products onto one f32.
 //
 // Layout. Tokens are the rows of the first product and the columns of the second: S^T = K Q^T and O^T = V^T P^T. A code page is read from
 // shared memory as it was stored: 16 bytes of a K row per thread are its operands of all eight steps, 16 bytes of a pair of V rows its
@@ -15,8 +21,8 @@
 // adds the two sums of its head; five to eight as they are, with a second product for the rests onto the same sums.
 //
 // What bounds it is instructions and their latency, not HBM: some 350 per page and warp, 152 of them widening codes, at 2.3 per cycle of an
-// SM with 12 warps. 64 lanes of 128 to 4096 tokens (32 query heads, 8 KV heads of 128; 158 MB) 45.6 us = 3470 GB/s, one of 131072
-// 43.5 us = 3470, 16 lanes of 1024 to 16384 with 64 heads 59.5 us = 2710 (the copy bandwidth is 6555).
+// SM with 12 warps. 64 lanes of 128 to 4096 tokens (32 query heads, 8 KV heads of 128; 158 MB) 47.9 us = 3300 GB/s, one of 131072
+// 45.2 us = 3340, 16 lanes of 1024 to 16384 with 64 heads 62.0 us = 2600 (the copy bandwidth is 6555).
 //
 // Work. The pages of all (lane, KV head) units in a row are cut into as many equal runs as there are warps, whatever the lengths of the
 // lanes: nobody waits for the longest. A warp takes its run by pages, or pairs of them, through a ring of cp.async copies that runs on
@@ -26,8 +32,8 @@
 // unit: 67 us against 51 for 64 lanes of 128 to 4096 tokens.) With PAIRS a warp has the registers to take two pages at once, whose scores,
 // reference and weights do not wait for each other: 45.8 us against 49.2 by single pages; a ring of two such steps does as well as longer ones.
 //
-// Scores are compared with a reference that is raised, with everything accumulated, only when one exceeds it by 2^kSlack: a few times per
-// run instead of once per page.
+// Scores, each with the size of its token's scales, are compared with a reference that is raised, with everything accumulated, only when one
+// exceeds it by 2^kSlack: a few times per run instead of once per page.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -49,9 +55,11 @@ constexpr int kWarps = 4, kResident = 3;  // of a CTA; CTAs of an SM: 168 regist
 constexpr int kDirectPages = 32;
 constexpr int kUnitPages = 6;  // what a unit costs beyond its pages, in pages
 constexpr int kPartPad = 4;  // of a head's part: reference, sum of weights, two unused
-constexpr float kSlack = 6.0f;
-constexpr float kWeightBits = 8.0f;  // weights are scaled by 2^8: at most 2^14 with the slack
-constexpr float kSmallestScale = 5.9604645e-8f;  // 2^-24, the smallest f16
+// The product of weight and largest |dv| of the token that set a head's reference is 2^11, of any other token at most 2^(11 + 3.75 + 0.09)
+// (0.09 by size_of), below what f16 holds.
+constexpr float kSlack = 3.75f;
+constexpr float kProductBits = 11.0f;
+constexpr float kRest = 2048.0f;  // PAIRS: rests are held times 2^11
 
 // What a CTA has of units that other CTAs have parts of: the end of one that began before it (part 0), the beginning of one that goes on
 // behind it (part 1).
@@ -213,8 +221,11 @@ __device__ __forceinline__ void store_out(const Q4Args& a, int D, int row, int k
   if (a.out_xh) a.out_xh[hand_off_cell(k >> 3, row, a.out_xh_nv, a.q_heads * (D / 8)) + (k & 7)] = half_sat(val);
 }
 
-// What V scales are multiplied by, of which no |dv| exceeds the power of two `top`: 1 / top, as far as f16 holds it.
-__device__ __forceinline__ __half2 scale_to_range(float top) { return __float2half2_rn(fminf(1.0f / top, 32768.0f)); }
+// log2 of an f16 number that is not negative, plus 15: its bits as a number, over 1024. Exact at powers of two, up to 0.09 too large
+// between them and, below 2^-14, by what keeps it from falling under 0.
+__device__ __forceinline__ float size_of(uint32_t bits, unsigned place) {  // place: 0x7410 for the low half of `bits`, 0x7432 for the high one
+  return fmaf(__uint_as_float(__byte_perm(bits, 0x4B000000u, place)), 1.0f / 1024.0f, -8192.0f);  // 2^23 + bits
+}
 
 template <int D, bool PAIRS>
 struct Q4Cfg {
@@ -437,17 +448,15 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
           }
     }
     float o[2 * NB][4];
-    float ref[MINE], limit[MINE], sub[MINE], weight[MINE];  // reference, score that raises it, what weights' exponents are less, this thread's sum of weights
+    float ref[MINE], limit[MINE], sub[MINE], weight[MINE];  // reference, what raises it, what weights' exponents are less, this thread's sum of weights
 #pragma unroll
     for (int m = 0; m < MINE; ++m) {
       ref[m] = limit[m] = -INFINITY;
-      sub[m] = -kWeightBits;  // for as long as every score is -inf or NaN
+      sub[m] = -(kProductBits + 15.0f);  // for as long as every score is -inf or NaN
       weight[m] = 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-    float top_scale = kSmallestScale;  // power of two that no |dv| so far exceeds
-    __half2 top_half = __float2half2_rn(top_scale), to_range = scale_to_range(top_scale);
     // this run's positions of the unit, and the pages of it without a masked token
     const int end_of_run = min(run.span.end, run.page1 * kPage), inner0 = (run.span.begin + kPage - 1) / kPage, inner1 = end_of_run / kPage;
 
@@ -531,39 +540,37 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
           }
         }
       }
-      auto largest_scale = [&](auto&& of) {
-        __half2 largest = __float2half2_rn(0.0f);
-#pragma unroll
-        for (int u = 0; u < PAGES; ++u)
-#pragma unroll
-          for (int i = 0; i < NB / 2; ++i) largest = __hmax2(largest, __hmax2(of(__habs2(halves(dv_lo[u][i]))), of(__habs2(halves(dv_hi[u][i])))));
-        return largest;
-      };
-      __half2 largest = largest_scale([](__half2 d) { return d; });
-      bool rises = !__hble2(largest, top_half);
-#pragma unroll
-      for (int u = 0; u < PAGES; ++u)
-#pragma unroll
-        for (int m = 0; m < MINE; ++m) rises = rises || !(s_lo[u][m] <= limit[m]) || !(s_hi[u][m] <= limit[m]);
-      if (__any_sync(0xffffffffu, rises)) {
-        // an infinite scale spoils the columns of its block, and nothing else: infinity times 0 takes no part in a maximum
-        largest = largest_scale([](__half2 d) { return __hmul2(d, __hle2(d, __float2half2_rn(65504.0f))); });
-        float scale = fmaxf(__low2float(largest), __high2float(largest)), shrink = 1.0f;
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) scale = fmaxf(scale, __shfl_xor_sync(0xffffffffu, scale, off));
-        if (scale > top_scale) {
-          top_scale = __uint_as_float((__float_as_uint(scale) + 0x7fffffu) & 0x7f800000u);  // the power of two at or above it
-          top_half = __float2half2_rn(top_scale);
-          const __half2 range = scale_to_range(top_scale);
-          shrink = __low2float(range) / __low2float(to_range);
-          to_range = range;
+      // The size of a token: its largest |dv| of any block, as a logarithm.
+      auto sizes_of = [&](int u, auto&& of, float& lo, float& hi) {
+        __half2 most_lo = of(__habs2(halves(dv_lo[u][0]))), most_hi = of(__habs2(halves(dv_hi[u][0])));
+        if constexpr (NB == 4) {
+          most_lo = __hmax2(most_lo, of(__habs2(halves(dv_lo[u][1]))));
+          most_hi = __hmax2(most_hi, of(__habs2(halves(dv_hi[u][1]))));
         }
+        const uint32_t both = bits(__hmax2(__lows2half2(most_lo, most_hi), __highs2half2(most_lo, most_hi)));
+        lo = size_of(both, 0x7410u);
+        hi = size_of(both, 0x7432u);
+      };
+      bool rises = false;
+#pragma unroll
+      for (int u = 0; u < PAGES; ++u) {
+        float lo, hi;
+        sizes_of(u, [](__half2 d) { return d; }, lo, hi);
+#pragma unroll
+        for (int m = 0; m < MINE; ++m) rises = rises || !(s_lo[u][m] + lo <= limit[m]) || !(s_hi[u][m] + hi <= limit[m]);
+      }
+      if (__any_sync(0xffffffffu, rises)) {
         float f[MINE];
 #pragma unroll
         for (int m = 0; m < MINE; ++m) {
           float most = -INFINITY;
 #pragma unroll
-          for (int u = 0; u < PAGES; ++u) most = fmaxf(most, fmaxf(s_lo[u][m], s_hi[u][m]));
+          for (int u = 0; u < PAGES; ++u) {
+            // an infinite scale spoils the columns of its block, and nothing else: it takes no part in the token's size
+            float lo, hi;
+            sizes_of(u, [](__half2 d) { return __halves2half2(__hisinf(__low2half(d)) ? __half() : __low2half(d), __hisinf(__high2half(d)) ? __half() : __high2half(d)); }, lo, hi);
+            most = fmaxf(most, fmaxf(s_lo[u][m] + lo, s_hi[u][m] + hi));
+          }
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
           f[m] = 1.0f;
@@ -571,10 +578,9 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
             f[m] = exp2_flushed(ref[m] - most);
             ref[m] = most;
             limit[m] = most + kSlack;
-            sub[m] = most - kWeightBits;
+            sub[m] = most - (kProductBits + 15.0f);
           }
           weight[m] *= f[m];
-          f[m] *= shrink;
         }
 #pragma unroll
         for (int i = 0; i < 2 * NB; ++i) {
@@ -583,8 +589,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
       }
 #pragma unroll
       for (int u = 0; u < PAGES; ++u) {
-        // Weights, and their products with the V scales as value and rest, transposed into operand order. All in f16: w is the weight's value
-        // and x its rest, w * d rounds to the product's value, and fma gives what that leaves out exactly, to which x * d is added.
+        // Weights, and their products with the V scales as value and rest, transposed into operand order.
         uint32_t pf[PAIRS ? 1 : 2][NB][2];
         float p_lo[MINE], p_hi[MINE];
 #pragma unroll
@@ -593,40 +598,25 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
           p_hi[m] = exp2_flushed(s_hi[u][m] - sub[m]);
           weight[m] += p_lo[m] + p_hi[m];
         }
-        auto rest_of = [](float v0, float v1, __half2 value) { return __floats2half2_rn(v0 - __low2float(value), v1 - __high2float(value)); };
-        if constexpr (PAIRS) {
-          const __half2 w = __floats2half2_rn(p_lo[0], p_hi[0]), x = rest_of(p_lo[0], p_hi[0], w);
-          const __half2 lo = __lows2half2(w, x), hi = __highs2half2(w, x), to_rest = __floats2half2_rn(0.0f, 1.0f);
-          // (w, x) * d, rounded; what the first product's rounding leaves out is added to the second
-          auto both = [&](__half2 wx, __half2 d) {
-            const __half2 rounded = __hmul2(wx, d);
-            return bits(__hfma2(__low2half2(__hfma2(wx, d, __hneg2(rounded))), to_rest, rounded));
-          };
 #pragma unroll
-          for (int i = 0; i < NB / 2; ++i) {
-            const __half2 d_lo = __hmul2(halves(dv_lo[u][i]), to_range), d_hi = __hmul2(halves(dv_hi[u][i]), to_range);
-            pf[0][2 * i][0] = transpose8(both(lo, __low2half2(d_lo)));
-            pf[0][2 * i][1] = transpose8(both(hi, __low2half2(d_hi)));
-            pf[0][2 * i + 1][0] = transpose8(both(lo, __high2half2(d_lo)));
-            pf[0][2 * i + 1][1] = transpose8(both(hi, __high2half2(d_hi)));
-          }
-        } else {
-          auto product = [](__half2 w, __half2 x, __half2 d, __half2& value, __half2& rest) {
-            value = __hmul2(w, d);
-            rest = __hfma2(x, d, __hfma2(w, d, __hneg2(value)));
-          };
-          const __half2 w_lo = __floats2half2_rn(p_lo[0], p_lo[1]), x_lo = rest_of(p_lo[0], p_lo[1], w_lo);
-          const __half2 w_hi = __floats2half2_rn(p_hi[0], p_hi[1]), x_hi = rest_of(p_hi[0], p_hi[1], w_hi);
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {  // two heads at a time
-            const __half2 d_lo = __hmul2(halves(dv_lo[u][b / 2]), to_range), d_hi = __hmul2(halves(dv_hi[u][b / 2]), to_range);
-            __half2 value_lo, rest_lo, value_hi, rest_hi;
-            product(w_lo, x_lo, b & 1 ? __high2half2(d_lo) : __low2half2(d_lo), value_lo, rest_lo);
-            product(w_hi, x_hi, b & 1 ? __high2half2(d_hi) : __low2half2(d_hi), value_hi, rest_hi);
-            pf[0][b][0] = transpose8(bits(value_lo));
-            pf[0][b][1] = transpose8(bits(value_hi));
-            pf[1][b][0] = transpose8(bits(rest_lo));
-            pf[1][b][1] = transpose8(bits(rest_hi));
+        for (int b = 0; b < NB; ++b) {
+          const float2 lo = __half22float2(halves(dv_lo[u][b / 2])), hi = __half22float2(halves(dv_hi[u][b / 2]));
+          const float d0 = b & 1 ? lo.y : lo.x, d1 = b & 1 ? hi.y : hi.x;
+          if constexpr (PAIRS) {
+            auto both = [](float x) {
+              const float value = __half2float(__float2half_rn(x));
+              return transpose8(bits(__floats2half2_rn(value, (x - value) * kRest)));
+            };
+            pf[0][b][0] = both(p_lo[0] * d0);
+            pf[0][b][1] = both(p_hi[0] * d1);
+          } else {
+            auto both = [&](float x0, float x1, int i) {  // of two heads
+              const __half2 value = __floats2half2_rn(x0, x1);
+              pf[0][b][i] = transpose8(bits(value));
+              pf[1][b][i] = transpose8(bits(__floats2half2_rn(x0 - __low2float(value), x1 - __high2float(value))));
+            };
+            both(p_lo[0] * d0, p_lo[1] * d0, 0);
+            both(p_hi[0] * d1, p_hi[1] * d1, 1);
           }
         }
         __align__(16) uint32_t w[2][NB];  // of tokens 2 t and 2 t + 1, and of those eight further
@@ -650,7 +640,6 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
     }
 
     // a whole unit is written, a part of one kept for the end
-    const float back = 1.0f / __low2float(to_range);  // the weights' own 2^kWeightBits cancels against that of their sum
     const bool begins = run.page0 == run.span.first, ends = run.page1 == run.span.first + run.span.pages;
     const int record = 2 * warp + (begins ? 1 : 0);
     if (lane == 0 && !(begins && ends)) records[record] = Record{1, ends, run.lane, head0, live_heads, run.stop + (run.span.first + run.span.pages - run.page1)};
@@ -659,11 +648,11 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) weight[m] += __shfl_xor_sync(0xffffffffu, weight[m], off);
       const int h = PAIRS ? t : 2 * t + m;
-      const float f = begins && ends ? (weight[m] == 0.0f ? 0.0f : back / weight[m]) : back;
+      const float f = begins && ends ? (weight[m] == 0.0f ? 0.0f : 1.0f / weight[m]) : 1.0f;  // the powers of two in both cancel
       float* dst = sums + (record * Cfg::kHeads + h) * Cfg::kPitch + g;
 #pragma unroll
       for (int i = 0; i < 4 * NB; ++i) {  // columns 8 i + g
-        const float val = (PAIRS ? o[i / 2][2 * (i & 1)] + o[i / 2][2 * (i & 1) + 1] : o[i / 2][2 * (i & 1) + m]) * f;
+        const float val = (PAIRS ? fmaf(o[i / 2][2 * (i & 1) + 1], 1.0f / kRest, o[i / 2][2 * (i & 1)]) : o[i / 2][2 * (i & 1) + m]) * f;
         if (!(begins && ends)) dst[8 * i] = val;
         else if (h < live_heads) store_out(a, D, run.lane, (head0 + h) * D + 8 * i + g, val);
       }
