@@ -1010,22 +1010,32 @@ __device__ __forceinline__ void cp_async16_or_zero(void* smem_dst, const void* g
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(gmem_src), "r"(live ? 16 : 0));
 }
 
-// The 4-bit tier's rows (kv_q4.cuh) as f16 values in the operand layout. Rows outside [begin, end) of the page positions that start at
-// `base` come out as zeros of V, whatever they hold.
+// The 4-bit tier's rows (kv_q4.cuh) as f16 values in the operand layout, rounded to 11 bits; with `eighths` an eighth of them, which no scale
+// takes out of the range of f16. Rows outside [begin, end) of the page positions that start at `base` come out as zeros of V, whatever they
+// hold. True where this thread has met a scale that whole values may overflow with.
 template <int D>
-__device__ __forceinline__ void widen_q4_step(const unsigned char* raw, unsigned char* wide, int base, int begin, int end) {
+__device__ __forceinline__ bool widen_q4_step(const unsigned char* raw, unsigned char* wide, int base, int begin, int end, bool eighths) {
   constexpr int NB = D / 32, RECORD = kPageTokens * NB * 18, CODES = kPageTokens * D / 2, SIDE = kChunkTokens * D * 2;
-  auto two = [](uint32_t w, bool low) {  // bits 0-3 or 4-7 of both halves -> codes less 8
+  const float part = eighths ? 0.125f : 1.0f;
+  const __half2 low_times = __float2half2_rn(part), low_less = __float2half2_rn(-1032.0f * part), high_times = __float2half2_rn(0.0625f * part),
+                high_less = __float2half2_rn(-72.0f * part);
+  auto two = [&](uint32_t w, bool low) {  // bits 0-3 or 4-7 of both halves -> codes less 8, exact
     uint32_t bits = (w & (low ? 0x000F000Fu : 0x00F000F0u)) | 0x64006400u;
     const __half2 h = *reinterpret_cast<__half2*>(&bits);
-    return low ? __hsub2(h, __floats2half2_rn(1032.0f, 1032.0f)) : __hfma2(h, __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-72.0f, -72.0f));
+    return low ? __hfma2(h, low_times, low_less) : __hfma2(h, high_times, high_less);
+  };
+  bool overflows = false;
+  auto scale_of = [&](const unsigned char* record, int row, int b, bool live) {
+    const __half d = reinterpret_cast<const __half*>(record + CODES)[row % kPageTokens * NB + b];
+    overflows = overflows || (live && __hgt(__habs(d), __float2half_rn(8188.0f)));  // 65504 / 8
+    return d;
   };
   auto word = [](__half2 h) { return *reinterpret_cast<uint32_t*>(&h); };
   for (int i = threadIdx.x; i < kChunkTokens * 4 * NB; i += 128) {  // a K word: eight values
     const int row = i / (4 * NB), at = i % (4 * NB), t = at / NB, b = at % NB;
     const unsigned char* record = raw + row / kPageTokens * RECORD;
     const uint32_t w = *reinterpret_cast<const uint32_t*>(record + row % kPageTokens * (D / 2) + at * 4);
-    const __half2 d = __half2half2(reinterpret_cast<const __half*>(record + CODES)[row % kPageTokens * NB + b]);
+    const __half2 d = __half2half2(scale_of(record, row, b, base + row >= begin && base + row < end));
     *reinterpret_cast<uint4*>(wide + swizzled_offset<D>(row, 4 * b + t)) =
         make_uint4(word(__hmul2(two(w, true), d)), word(__hmul2(two(w, false), d)), word(__hmul2(two(w >> 8, true), d)), word(__hmul2(two(w >> 8, false), d)));
   }
@@ -1039,7 +1049,8 @@ __device__ __forceinline__ void widen_q4_step(const unsigned char* raw, unsigned
     for (int u = 0; u < 2; ++u) {
       const int row = row0 + u;
       const bool live = base + row >= begin && base + row < end;
-      const __half2 d = live ? __half2half2(reinterpret_cast<const __half*>(record + CODES)[row % kPageTokens * NB + b]) : __floats2half2_rn(0.0f, 0.0f);
+      const __half d_row = scale_of(record, row, b, live);
+      const __half2 d = live ? __half2half2(d_row) : __floats2half2_rn(0.0f, 0.0f);
       uint32_t x[4];  // the block's codes of columns g = 2 q and 2 q + 1 of every eight
 #pragma unroll
       for (int q = 0; q < 4; ++q) x[q] = __byte_perm(w[2 * q], w[2 * q + 1], u ? 0x7632 : 0x5410);
@@ -1052,6 +1063,7 @@ __device__ __forceinline__ void widen_q4_step(const unsigned char* raw, unsigned
       }
     }
   }
+  return overflows;
 }
 
 template <int D, bool BF16, int TIER>
@@ -1136,6 +1148,7 @@ __global__ void __launch_bounds__(128, TIER == kChunkHalves ? 3 : 2) attention_c
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
   float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.0f, l_hi = 0.0f;
+  bool eighths = false;  // 4-bit tier: K and V are taken as eighths from here on, the same for the whole CTA
 
   for (int step = 0; step < steps; ++step) {
     cp_async_wait<0>();
@@ -1164,8 +1177,17 @@ __global__ void __launch_bounds__(128, TIER == kChunkHalves ? 3 : 2) attention_c
     }
     if constexpr (Q4) {
       unsigned char* wide = smem + 2 * Cfg::kStage;
-      widen_q4_step<D>(raw, wide, (first_page + step * kChunkPages) * kPageTokens, begin, end);
-      __syncthreads();
+      const int at = (first_page + step * kChunkPages) * kPageTokens;
+      const bool overflows = widen_q4_step<D>(raw, wide, at, begin, end, eighths);
+      if (__syncthreads_or(overflows) && !eighths) {
+        eighths = true;
+#pragma unroll
+        for (int i = 0; i < DTILES; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[i][j] *= 0.125f;
+        widen_q4_step<D>(raw, wide, at, begin, end, true);
+        __syncthreads();
+      }
       ks_page = wide;
       vs_page = wide + Cfg::kSide;
     }
@@ -1189,6 +1211,12 @@ __global__ void __launch_bounds__(128, TIER == kChunkHalves ? 3 : 2) attention_c
         const float2 sc = *reinterpret_cast<const float2*>(scales + n * 8 + 2 * t);
         s[n][0] *= sc.x; s[n][1] *= sc.y; s[n][2] *= sc.x; s[n][3] *= sc.y;
       }
+    }
+    if (Q4 && eighths) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] *= 8.0f;
     }
     if (base < full_begin || base + kChunkTokens > full_end) {
 #pragma unroll
@@ -1250,7 +1278,7 @@ __global__ void __launch_bounds__(128, TIER == kChunkHalves ? 3 : 2) attention_c
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     if (!(h ? live_hi : live_lo)) continue;
-    const float l = h ? l_hi : l_lo, inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float l = h ? l_hi : l_lo, inv = l > 0.0f ? (Q4 && eighths ? 8.0f : 1.0f) / l : 0.0f;
     const size_t row = (size_t)lane_id * T + (h ? token_hi : token_lo);
     const int head = kv_head * G + (h ? row_hi : row_lo) % G;
 #pragma unroll
