@@ -298,7 +298,7 @@ ETC_API etc_status etc_sample_row(etc_runtime* rt, const float* d_logits, int64_
  *   d_top_tokens / d_top_logprobs [rows, top]: the most likely tokens, largest first, of equal logits the lower token first, and
  *                   their log probabilities             (top in 0..min(32, vocab); NULL with 0)
  * -inf logits (barred tokens) have log probability -inf; a row of nothing else has NaN log probabilities and entropy and its first
- * tokens as alternatives. Sums are f32 within some 250 values and f64 above. Asynchronous, capturable, nothing allocated. A
+ * tokens as alternatives. Sums are f32 over at most 200 additions in a row and f64 above. Asynchronous, capturable, nothing allocated. A
  * target >= vocab (its log probability is NaN) is reported at the next synchronising call as ETC_EXECUTION "logprobs: target {t}
  * is outside 0..{vocab}", a NaN or +inf logit as "logprobs: logit {i} of row {r} is NaN or +inf" (that row's results mean nothing). */
 ETC_API etc_status etc_logprobs_into(etc_runtime* rt, const float* d_logits, int64_t rows, int64_t vocab, int64_t row_stride,
