@@ -489,8 +489,8 @@ etc_status check_paged(etc_runtime* rt, etc_pool* pool, int layer) {
 
 etc_status check_decode_supported(const PoolView& view, int q_heads) {
   if (view.dtype == ETC_KV_Q4 ? attention_q4_supported(view, q_heads) : attention_mma_supported(view, q_heads, 1)) return ETC_OK;
-  return fail(ETC_UNSUPPORTED, "kv attention: the tensor-core decode kernel needs an f16/bf16 pool with 16-token pages, head "
-                               "dim 64 or 128 and at most 16 query heads per kv head");
+  return fail(ETC_UNSUPPORTED, "kv attention: the tensor-core decode kernel needs an f16, bf16, u8 or q4 pool with 16-token pages, "
+                               "head dim 64 or 128 and at most 16 query heads per kv head");
 }
 
 // Attention of one query token per lane, by the tier's kernel.

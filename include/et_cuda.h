@@ -348,7 +348,7 @@ ETC_API etc_status etc_kv_attention_into(etc_runtime* rt, etc_pool* pool, int la
 ETC_API etc_status etc_kv_append_into(etc_runtime* rt, etc_pool* pool, int layer, etc_seq* const* seqs, int batch,
                                       int active, int advance, const float* d_k, const float* d_v, int tokens,
                                       int64_t pool_window);
-/* kv_attention_into for one-token decode steps on the tensor-core flash-decoding kernel (f16/bf16 pools,
+/* kv_attention_into for one-token decode steps on the tensor-core flash-decoding kernel (f16, bf16, u8, q4 pools,
  * 16-token pages, head dim 64/128): d_q f32 [batch, q_heads, head_dim], d_k/d_v f32 [batch, kv_heads,
  * head_dim] (may both be NULL when the step's rows were already appended), d_out like d_q. Same page
  * allocation, masking and window rules as etc_kv_attention_into; results within the f16 tolerance. */
