@@ -546,7 +546,8 @@ struct ScoreRequest {
 // Rows whose logits exist at a time (131 MB of a vocabulary of 128256): enough for the large-batch linear to run at its rate.
 constexpr int64_t kScoreRows = 256;
 
-// Device buffers of a scoring step, kept from one to the next: [logits][linear scratch][targets][log probabilities][entropy][top tokens][top].
+// Device buffers of a scoring step, kept from one to the next: [logits][linear scratch] (none for one token per lane, whose logits and scratch are
+// the step's own) [targets][log probabilities][entropy][top tokens][top].
 struct ScoreBuffers {
   float* logits;
   void* scratch;
@@ -555,10 +556,10 @@ struct ScoreBuffers {
   uint32_t* top_tokens;
   float* top_logprobs;
 };
-etc_status score_buffers(etc_decoder* d, int64_t rows, int top, ScoreBuffers* out) {
-  const int64_t at_once = std::min(std::max<int64_t>(kScoreRows, d->cfg.batch), rows);
+etc_status score_buffers(etc_decoder* d, int active, int advance, int top, ScoreBuffers* out) {
+  const int64_t rows = (int64_t)active * advance, at_once = advance == 1 ? 0 : std::min(std::max<int64_t>(kScoreRows, d->cfg.batch), rows);
   size_t scratch = 0;
-  if (d->tiled)
+  if (d->tiled && at_once > 0)
     for (int64_t v : {at_once, rows % at_once}) scratch = std::max(scratch, v > 0 ? tiled_scratch_bytes(d->t_head->tiled, v, d->rt->sm_count) : 0);
   size_t offsets[7], bytes = 0;
   const size_t sizes[7] = {(size_t)at_once * d->cfg.vocab * 4, scratch, (size_t)rows * 4, (size_t)rows * 4, (size_t)rows * 4, (size_t)rows * top * 4, (size_t)rows * top * 4};
@@ -782,7 +783,7 @@ etc_status execute_impl(etc_decoder* dec, etc_pool* pool, etc_seq* const* seqs, 
   if (request) {
     ScoreBuffers buffers;
     const int64_t rows = (int64_t)active * advance;
-    st = score_buffers(dec, rows, request->top, &buffers);
+    st = score_buffers(dec, active, advance, request->top, &buffers);
     if (st == ETC_OK) st = enqueue_score(ctx, active, *request, buffers);
     if (st != ETC_OK) return abort_with(st);
     score_results.resize((size_t)rows * (2 + 2 * request->top));

@@ -16,3 +16,22 @@ def test_the_decode_kernels_name_the_tiers_they_take():
         rt.paged_attention_into(pool, 0, lanes, tables, 1, 4, q, 4, 1.0, out, empty(1 << 20), 1 << 20)
     for tier in (et.KV_F16, et.KV_BF16, et.KV_U8, et.KV_Q4):
         et.NativeKvPool(rt, 1, 2, 64, 64, 16, tier).attention_scratch_bytes(1, 4, 4)
+
+
+@pytest.mark.parametrize("exact", [True, False])
+def test_scoring_token_by_token_holds_no_logits_of_its_own(exact):
+    import oracle as orc
+    from tests import helpers
+    from tests.test_gpu_long_context import SMALL, SMALL_Q, make
+
+    cfg = SMALL if exact else SMALL_Q
+    dec, pool, _ = make(cfg, helpers.make_weights(cfg, seed=1, codec=0 if exact else orc.Q4_0), 4, et.KV_F16, exact, None)
+    seqs, rt = [pool.makeSequence() for _ in range(4)], runtime()
+    before = rt.memory_bytes
+    first = dec.score(pool, seqs, np.ones((4, 1)), np.full((4, 1), 5), top=2)
+    assert rt.memory_bytes - before < 4 * cfg["vocab"]  # less than a row of logits
+    dec.score(pool, seqs, np.ones((4, 3)), np.ones((4, 3)), top=2)
+    assert rt.memory_bytes - before > 12 * 4 * cfg["vocab"]
+    again = [pool.makeSequence() for _ in range(4)]
+    for a, b in zip(first, dec.score(pool, again, np.ones((4, 1)), np.full((4, 1), 5), top=2)):
+        np.testing.assert_array_equal(a, b)
