@@ -1318,7 +1318,7 @@ etc_status etc_decoder_score(etc_decoder* dec, etc_pool* pool, etc_seq* const* s
   if (!valid_decoder(dec)) return fail(ETC_INVALID_HANDLE, "decoder handle is invalid or destroyed");
   if (!h_targets || !h_logprobs || (top > 0 && (!h_top_tokens || !h_top_logprobs)))
     return fail(ETC_INVALID_ARGUMENT, "score: targets, log probabilities and buffers for the alternatives must be given");
-  if (dec->vocab_global > 0 && dec->tp_world > 1) return fail(ETC_UNSUPPORTED, "score: a vocabulary-parallel head holds a part of every distribution only");
+  if (dec->vocab_global > 0 && (dec->tp_world > 1 || dec->vocab_global != dec->cfg.vocab)) return fail(ETC_UNSUPPORTED, "score: a vocabulary-parallel head holds a part of every distribution only");
   ETC_TRY(validate_logprobs(dec->cfg.vocab, top));
   const bool sized = active >= 0 && active <= dec->cfg.batch && advance >= 0 && advance <= dec->max_advance;  // others are refused below
   for (int64_t i = 0; sized && i < (int64_t)active * advance; ++i)

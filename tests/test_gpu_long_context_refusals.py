@@ -35,3 +35,26 @@ def test_scoring_token_by_token_holds_no_logits_of_its_own(exact):
     again = [pool.makeSequence() for _ in range(4)]
     for a, b in zip(first, dec.score(pool, again, np.ones((4, 1)), np.full((4, 1), 5), top=2)):
         np.testing.assert_array_equal(a, b)
+
+
+def test_scores_of_a_part_of_the_vocabulary_are_refused():
+    """Also where the decoder of that part stands alone: its logits are no distribution."""
+    from tests import helpers
+    from tests.test_gpu_long_context import SMALL
+
+    half = dict(SMALL, vocab=750)
+    w = helpers.make_weights(SMALL, seed=1)
+    for first, whole in ((0, False), (750, False), (0, True)):
+        cfg = SMALL if whole else half
+        dec = et.Executable(runtime(), **cfg, batch=1, max_tokens=64, exact=True, vocab_global=1500, head_first_row=first)
+        helpers.load_into(dec, dict(w, head=w["head"][first:first + cfg["vocab"]]))
+        dec.finalize()
+        pool = et.NativeKvPool(runtime(), cfg["layers"], cfg["kv_heads"], cfg["head_dim"], 64, 16, et.KV_F32)
+        seqs = [pool.makeSequence()]
+        if whole:
+            dec.score(pool, seqs, [[3]], [[4]])
+            continue
+        with pytest.raises(et.BackendError, match="vocabulary-parallel head"):
+            dec.score(pool, seqs, [[3]], [[4]])
+        assert seqs[0].cursor == 0
+        dec.execute(pool, seqs, [[3]])
