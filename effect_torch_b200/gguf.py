@@ -138,9 +138,9 @@ def llama_geometry(f: GgufFile) -> dict:
 def llama_rope(f: GgufFile, geometry: dict, layout: int):
     """How a Llama-family file has its positions rotated, as a RopeConfig: `<arch>.rope.dimension_count` (part of the head) and the
     `<arch>.rope.scaling.*` keys (none, linear, yarn). None where it asks for nothing beyond whole heads at freq_base; a kind of scaling
-    that is not known, or lacks what it needs, is left out with a warning. (The llama3 rule comes as divisors per pair, in the tensor
-    rope_freqs.weight.)"""
-    from . import rope_config
+    that is not known, or lacks what it needs, and values that no rotation has (half a pair, a factor below 1) are left out with a
+    warning. (The llama3 rule comes as divisors per pair, in the tensor rope_freqs.weight: llama_rope_divisors.)"""
+    from . import rope_config, rope_frequencies
 
     meta = {m["key"]: m.get("value") for m in f.metadata if not m["array"]}
     key = lambda name, default=None: meta.get(f"{f.architecture}.rope.{name}", default)
@@ -159,10 +159,31 @@ def llama_rope(f: GgufFile, geometry: dict, layout: int):
             if key(name) is not None:
                 rule[option] = float(key(name))
         attention = float(key("scaling.attn_factor", 1.0))  # on top of the rule's own
-        rule["attention_factor"] = attention * (0.1 * math.log(factor) + 1.0) if attention != 1.0 else 0.0
+        rule["attention_factor"] = attention * (0.1 * math.log(factor) + 1.0) if attention != 1.0 and factor > 0 else 0.0
     elif kind not in ("none", "linear"):
         warnings.warn(f"gguf: rope scaling {kind!r} is not known or lacks its original context length; positions are not scaled", stacklevel=3)
-    return rope_config(geometry["head_dim"], theta=geometry["rope_theta"], layout=layout, **rule) if rule else None
+    if not rule:
+        return None
+    config = rope_config(geometry["head_dim"], theta=geometry["rope_theta"], layout=layout, **rule)
+    try:
+        rope_frequencies(config)
+    except BackendError as error:
+        warnings.warn(f"gguf: the file's rope keys cannot be followed ({error}); whole heads are rotated and positions are not scaled", stacklevel=3)
+        return None
+    return config
+
+
+def llama_rope_divisors(f: GgufFile, pairs: int):
+    """The frequency divisor of each rotated pair, from the tensor rope_freqs.weight; None without it, and with a warning where it does not
+    hold one positive F32 number per pair."""
+    info = next((t for t in f.tensors if t.name == "rope_freqs.weight"), None)
+    if info is None:
+        return None
+    divisors = f.read_tensor(f.index(info.name)).view(np.float32) if info.codec == 0 else np.zeros(0, np.float32)
+    if divisors.size != pairs or not (np.isfinite(divisors) & (divisors > 0)).all():
+        warnings.warn(f"gguf: rope_freqs.weight does not hold {pairs} positive F32 divisors; positions are not scaled by it", stacklevel=3)
+        return None
+    return divisors
 
 
 def load_llama_decoder(rt, path: str, *, batch: int, max_tokens: int, block_size: int = 16, kv_dtype=None, exact: bool = False,
@@ -180,16 +201,12 @@ def load_llama_decoder(rt, path: str, *, batch: int, max_tokens: int, block_size
         g = llama_geometry(f)
         names = {t.name: i for i, t in enumerate(f.tensors)}
         layout = HALF_SPLIT if rope_layout is None else rope_layout
-        divisors = None
-        if "rope_freqs.weight" in names:
-            info = f.tensors[names["rope_freqs.weight"]]
-            if info.codec != 0:
-                raise BackendError(9, "gguf: rope_freqs.weight must be F32")
-            divisors = f.read_tensor(names["rope_freqs.weight"]).view(np.float32)
+        rope = llama_rope(f, g, layout)
+        divisors = llama_rope_divisors(f, (rope.rotary_dim if rope else g["head_dim"]) // 2)
         dec = Executable(rt, layers=g["layers"], d_model=g["d_model"], q_heads=g["q_heads"], kv_heads=g["kv_heads"], head_dim=g["head_dim"],
                          ffn=g["ffn"], vocab=g["vocab"], rms_eps=g["rms_eps"], rope_theta=g["rope_theta"],
                          rope_layout=layout, window=window, batch=batch, max_tokens=max_tokens, block_size=block_size,
-                         kv_dtype=KV_F16 if kv_dtype is None else kv_dtype, exact=exact, max_advance=max_advance, rope=llama_rope(f, g, layout),
+                         kv_dtype=KV_F16 if kv_dtype is None else kv_dtype, exact=exact, max_advance=max_advance, rope=rope,
                          rope_divisors=divisors)
 
         def bind(slot, layer, name):
