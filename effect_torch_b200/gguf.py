@@ -148,7 +148,7 @@ def llama_rope(f: GgufFile, geometry: dict, layout: int):
     rotary = int(key("dimension_count", geometry["head_dim"]))
     if rotary != geometry["head_dim"]:
         rule["rotary_dim"] = rotary
-    kind = key("scaling.type", "linear" if key("scale_linear") is not None else "none")
+    kind = key("scaling.type", "linear")  # a factor without a type is a linear one's
     factor = float(key("scaling.factor", key("scale_linear", 1.0))) or 1.0  # 0: not set
     original = float(key("scaling.original_context_length", meta.get(f"{f.architecture}.context_length", 0)))
     if kind == "linear" and factor != 1.0:

@@ -49,3 +49,12 @@ def test_divisors_of_a_file(tmp_path):
     for bad in (values[:31], np.where(np.arange(32) == 3, 0, values), np.where(np.arange(32) == 31, np.nan, values), -values):
         with pytest.warns(UserWarning, match="does not hold 32 positive F32 divisors"):
             assert divisors_of(tmp_path, bad, 32) is None
+
+
+@pytest.mark.parametrize("keys,factor", [({"llama.rope.scaling.factor": F32(4.0)}, 4.0), ({"llama.rope.scaling.factor": F32(4.0), "llama.rope.scale_linear": F32(2.0)}, 4.0),
+                                         ({"llama.rope.scaling.factor": F32(1.0)}, None), ({"llama.rope.scaling.factor": F32(0.0)}, None),
+                                         ({"llama.rope.scaling.type": TEXT("none"), "llama.rope.scaling.factor": F32(4.0)}, None)])
+def test_a_factor_without_a_type_is_linear(tmp_path, keys, factor):
+    config = rope_of(tmp_path, keys)
+    assert (config is None) == (factor is None)
+    assert config is None or (config.scaling, config.factor) == (et.ROPE_SCALINGS["linear"], factor)
