@@ -497,6 +497,8 @@ etc_status check_decode_supported(const PoolView& view, int q_heads) {
 etc_status decode_attention(etc_runtime* rt, const PoolView& view, const LaneInfo* d_lanes, const int* d_tables, int batch, int max_pages, const float* d_q,
                             int q_heads, double scale, int64_t op_window, float* d_out, float* d_scratch, size_t scratch_bytes) {
   auto check_scratch = [&](size_t needed) {
+    if (needed > 0 && reinterpret_cast<uintptr_t>(d_scratch) % alignof(float) != 0)
+      return fail(ETC_INVALID_ARGUMENT, "kv attention: scratch must lie on a 4-byte boundary");
     if (needed <= scratch_bytes && (needed == 0 || d_scratch)) return ETC_OK;
     return fail(ETC_INVALID_ARGUMENT, "kv attention: scratch holds " + std::to_string(scratch_bytes) + " bytes, " + std::to_string(needed) + " needed");
   };

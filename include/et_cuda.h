@@ -481,7 +481,8 @@ ETC_API etc_status etc_peer_allreduce_into(etc_runtime* rt, int rank, int world,
  * graph and replayed. d_lanes[i] = {cursor, advance (1 = live lane, 0 = padded), start (first resident position),
  * table_offset (index in d_tables of the block that holds position 0)}; lane i attends over positions [start, cursor +
  * advance) (further narrowed by op_window). max_pages bounds the pages any lane attends over and fixes the split plan;
- * d_scratch holds etc_paged_attention_scratch_bytes for that plan (of an f16, bf16 or u8 pool etc_kv_attention_plan(...).partial_bytes).
+ * d_scratch, on a 4-byte boundary, holds etc_paged_attention_scratch_bytes for that plan (of an f16, bf16 or u8 pool
+ * etc_kv_attention_plan(...).partial_bytes).
  * Needs an f16, bf16, u8 or q4 pool with 16-token pages. Over a q4 pool queries are held to 2^-22 (of their largest value 2^-38), the
  * products of softmax weights and V scales to 2^-22 or 2^-36 of the largest product of their head (2^-47 with up to four query heads per KV
  * head), everything else is f32; a lane may attend over no more than max_pages pages, as for the others. */

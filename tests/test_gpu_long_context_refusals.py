@@ -58,3 +58,22 @@ def test_scores_of_a_part_of_the_vocabulary_are_refused():
             dec.score(pool, seqs, [[3]], [[4]])
         assert seqs[0].cursor == 0
         dec.execute(pool, seqs, [[3]])
+
+
+@pytest.mark.parametrize("tier", [et.KV_F16, et.KV_U8, et.KV_Q4])
+def test_scratch_between_floats_is_refused(tier):
+    """Scratch is given in bytes, so that it may begin anywhere; partial sums in it are floats."""
+    rt = runtime()
+    pool = et.NativeKvPool(rt, 1, 2, 64, 64, 16, tier)
+    lanes, tables, q, out = dev(np.array([[0, 1, 0, 0]], np.int32)), dev(np.zeros(4, np.int32)), empty((1, 4, 64)), empty((1, 4, 64))
+    pages = 400
+    need = pool.attention_scratch_bytes(1, 4, pages)
+    assert need > 0
+    scratch = empty(need // 4 + 8)
+    for shift in (1, 2, 3):
+        with pytest.raises(et.BackendError, match="scratch must lie on a 4-byte boundary"):
+            rt.paged_attention_into(pool, 0, lanes, tables, 1, pages, q, 4, 1.0, out, scratch.data_ptr() + shift, need + 8)
+    rt.paged_append_into(pool, 0, lanes, tables, 1, 1, dev(np.ones((1, 2, 1, 64), np.float32)), dev(np.full((1, 2, 1, 64), 0.5, np.float32)))
+    rt.paged_attention_into(pool, 0, lanes, tables, 1, pages, q, 4, 1.0, out, scratch.data_ptr() + 4, need + 4)
+    rt.synchronize()
+    assert np.isfinite(out.cpu().numpy()).all()
