@@ -60,6 +60,8 @@ constexpr int kPartPad = 4;  // of a head's part: reference, sum of weights, two
 constexpr float kSlack = 3.75f;
 constexpr float kProductBits = 11.0f;
 constexpr float kRest = 2048.0f;  // PAIRS: rests are held times 2^11
+constexpr float kSizeZero = 15.0f;  // size_of(1)
+constexpr float kNoReference = -1e38f;  // any finite score raises it, and weights under it are 0
 
 // What a CTA has of units that other CTAs have parts of: the end of one that began before it (part 0), the beginning of one that goes on
 // behind it (part 1).
@@ -448,11 +450,10 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
           }
     }
     float o[2 * NB][4];
-    float ref[MINE], limit[MINE], sub[MINE], weight[MINE];  // reference, what raises it, what weights' exponents are less, this thread's sum of weights
+    float sub[MINE], weight[MINE];  // what weights' exponents are less than scores, by the reference; this thread's sum of weights
 #pragma unroll
     for (int m = 0; m < MINE; ++m) {
-      ref[m] = limit[m] = -INFINITY;
-      sub[m] = -(kProductBits + 15.0f);  // for as long as every score is -inf or NaN
+      sub[m] = kNoReference;
       weight[m] = 0.0f;
     }
 #pragma unroll
@@ -551,13 +552,14 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
         lo = size_of(both, 0x7410u);
         hi = size_of(both, 0x7432u);
       };
+      constexpr float kMost = kProductBits + kSizeZero + kSlack;  // of a weight's exponent and its token's size together
       bool rises = false;
 #pragma unroll
       for (int u = 0; u < PAGES; ++u) {
         float lo, hi;
         sizes_of(u, [](__half2 d) { return d; }, lo, hi);
 #pragma unroll
-        for (int m = 0; m < MINE; ++m) rises = rises || !(s_lo[u][m] + lo <= limit[m]) || !(s_hi[u][m] + hi <= limit[m]);
+        for (int m = 0; m < MINE; ++m) rises = rises || !(s_lo[u][m] - sub[m] + lo <= kMost) || !(s_hi[u][m] - sub[m] + hi <= kMost);
       }
       if (__any_sync(0xffffffffu, rises)) {
         float f[MINE];
@@ -574,11 +576,11 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
           f[m] = 1.0f;
-          if (most > limit[m]) {  // each head for itself: its result does not depend on the others
-            f[m] = exp2_flushed(ref[m] - most);
-            ref[m] = most;
-            limit[m] = most + kSlack;
-            sub[m] = most - (kProductBits + 15.0f);
+          if (most - sub[m] > kMost) {  // each head for itself: its result does not depend on the others
+            float to = most - (kProductBits + kSizeZero);
+            if (most - to > kProductBits + kSizeZero + 0.5f) to = most;  // scores so large that f32 does not resolve the difference
+            f[m] = exp2_flushed(sub[m] - to);
+            sub[m] = to;
           }
           weight[m] *= f[m];
         }
@@ -657,7 +659,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) attention_q4_kernel(Q4
         else if (h < live_heads) store_out(a, D, run.lane, (head0 + h) * D + 8 * i + g, val);
       }
       if (g == 0) {
-        refs[record * Cfg::kHeads + h] = ref[m];
+        refs[record * Cfg::kHeads + h] = sub[m];
         weights[record * Cfg::kHeads + h] = weight[m];
       }
     }

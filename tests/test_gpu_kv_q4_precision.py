@@ -118,3 +118,29 @@ def test_scales_below_the_normal_range_of_f16(q_heads):
     check(k, v * np.float32(2e-6), rng.normal(size=(q_heads, 128)).astype(np.float32), 0.1)
     v[..., 32:] *= np.float32(1e-5)
     check(k, v, rng.normal(size=(q_heads, 128)).astype(np.float32), 0.1)
+
+
+@pytest.mark.parametrize("q_heads", [1, 4, 8])
+@pytest.mark.parametrize("power", [10, 20, 22, 23, 24, 25, 26, 27, 28, 29, 31, 40, 60])
+@pytest.mark.parametrize("size", [1e-5, 1.0, 1e4])
+def test_scores_beyond_what_f32_resolves(q_heads, power, size):
+    """Scores of some 2^power that differ by a few units, or by what f32 keeps of them there: whatever the weights, a result is a mean of the
+    values, within a part in 2^18 of the largest (two splits and the sums' own roundings)."""
+    rng = np.random.default_rng(power)
+    n, D = 700, 64
+    k, v = np.zeros((1, n, D), np.float32), (size * np.exp(rng.normal(size=(1, n, 1))) * rng.normal(size=(1, n, D))).astype(np.float32)
+    k[..., 0], k[..., 32] = 1.0, rng.normal(size=n)
+    q = np.zeros((1, q_heads, D), np.float32)
+    q[..., 0], q[..., 32] = 2.0 ** power * 0.7, 20.0
+    cache = Cache([1], 1, D, spare=-(-n // PAGE) + 2)
+    runtime().paged_append_into(cache.pool, 0, lanes_of([[0, n, 0, 0]]), cache.tables, 1, n, dev(k[None].reshape(1, 1, n, D)), dev(v[None].reshape(1, 1, n, D)))
+    values = stored(v)[0]
+    fine = np.isfinite(values).all(0)  # with 1e4 some values leave the range that scales have: the columns of their blocks have no result
+    assert size == 1e4 or fine.all()
+    values = values[:, fine]
+    room = 2.0 ** -18 * np.abs(values).max(initial=0.0)
+    for pages in (44, 100):
+        got = attend(cache, q, 1.0, [(n - 1, 1, 0, 0)], pages)[0]
+        np.testing.assert_array_equal(np.isfinite(got), np.broadcast_to(fine, got.shape))
+        got = got[:, fine]
+        assert (got >= values.min(0) - room).all() and (got <= values.max(0) + room).all()
