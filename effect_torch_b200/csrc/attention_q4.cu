@@ -10,7 +10,7 @@
 // 2^-38 of the largest. For p * dv the power of two is that of the softmax: a head's reference is the largest (score + log2 of the token's
 // largest |dv|), not the largest score, so that the largest product is 2^11 or more whatever the scales are. Products are held to 2^-22 of themselves, or to
 // half of the smallest f16 number, 2^-36 of the largest one: a token whose weight is next to nothing adds that error once. With up to four heads
-// (below) rests have columns and sums of their own and are held times 2^11, which makes it 2^-47. (A reference of scores alone and one power of
+// (below) rests have columns and sums of their own and are held times 2^11, which makes it 2^-47. Scales below 2^-14 count as 2^-14 in this. (A reference of scores alone and one power of
 // two for all dv of a run were 2.3 us faster over 64 lanes, and off by 3 % in a block whose scales are 1e6 below another's, and by
 // 3e-6 to 5e-5 where one token draws most of the weight of 131072.) What remains is the tensor core's own sums, 16 products onto one f32.
 //
@@ -20,7 +20,7 @@
 // four (PAIRS) as (value, rest) pairs, so that the split costs no tensor instruction where columns would stay empty, and a thread
 // adds the two sums of its head; five to eight as they are, with a second product for the rests onto the same sums.
 //
-// What bounds it is instructions and their latency, not HBM: some 350 per page and warp, 152 of them widening codes, at 2.3 per cycle of an
+// What bounds it is instructions and their latency, not HBM: some 390 per page and warp, 152 of them widening codes, at 2.4 per cycle of an
 // SM with 12 warps. 64 lanes of 128 to 4096 tokens (32 query heads, 8 KV heads of 128; 158 MB) 47.9 us = 3300 GB/s, one of 131072
 // 45.2 us = 3340, 16 lanes of 1024 to 16384 with 64 heads 62.0 us = 2600 (the copy bandwidth is 6555).
 //
@@ -50,8 +50,11 @@ namespace {
 constexpr int kPage = 16;
 constexpr int kStages = 2;
 constexpr int kWarps = 4, kResident = 3;  // of a CTA; CTAs of an SM: 168 registers for a thread
-// Tables of up to 32 pages take a CTA per unit: 512 tokens of 1, 8 and 32 sequences (8 KV heads of 128) 8.3, 10.1 and 11.8 us against
-// 9.7, 11.4 and 17.7 by runs; 1024 tokens 11.2, 15.1 and 17.3 against 10.9, 12.0 and 20.5.
+// Tables of up to 32 pages take a CTA per unit. Both ways (directly / by runs, us) for sequences of half to all of 512, 768 and 1024 tokens, 32 heads over 8 of 128: one
+// sequence 8.5 / 9.7, 9.9 / 9.9, 11.3 / 11.3; eight 10.4 / 11.3, 12.9 / 11.2, 15.4 / 11.7; 32 sequences 12.4 / 17.8, 15.4 / 20.0, 18.4 / 20.5. 64
+// heads: one 11.6 / 11.3, 13.9 / 11.8; eight 14.1 / 13.3, 17.4 / 14.5; 32 16.2 / 19.8, 20.7 / 22.2, 24.8 / 24.2. 4 heads over 1 of 64: 6.1 / 7.8, 7.0 /
+// 8.2, 7.9 / 8.2. The pages alone do not decide it: many sequences and small models are up to a quarter slower from 33 to 64 pages than a CTA
+// per unit would be, eight sequences of 64 heads 6 % at 32 pages than runs would.
 constexpr int kDirectPages = 32;
 constexpr int kUnitPages = 6;  // what a unit costs beyond its pages, in pages
 constexpr int kPartPad = 4;  // of a head's part: reference, sum of weights, two unused

@@ -8,11 +8,12 @@
 // shuffles, through shared memory and, where several CTAs share a row, through the cluster's. The alternatives need no second
 // pass either: the n-th largest of the maxima of 32 groups of threads (a 64-bit key of value and inverted token, so that no two are
 // equal) is a lower bound of the n-th largest key. Only threads whose own maximum reaches it can hold an alternative; a warp
-// looks at each such thread's values again (some hundred, from L2), lists those that reach the bound, and the list is ranked by
+// looks at each such thread's values again (some hundred; from L2 where few rows are in flight, else from HBM), lists those that reach the bound, and the list is ranked by
 // counting. Should the list overflow (an order of logits made for it), the alternatives are found one after the other instead.
 //
-// Bound by HBM where rows are many, 2048 of 128256 (1.05 GB) 163.5 us = 6.4 TB/s of a copy's 6.55; by latency where they are
-// few, one with 20 alternatives 10.7 us, 32 with 5 alternatives 11.5.
+// Bound by HBM where rows are many, 2048 of 128256 (1.05 GB) 160 to 171 us (boxes differ) = 6.15 to 6.55 TB/s of a copy's 6.55; by latency where
+// they are few, one with 20 alternatives 10.8 us, 32 with 5 alternatives 11.5. Many rows with alternatives read part of the row twice: 2048 with 20 take
+// 288 us, with 32 428.
 //
 // Sums are f32 within a batch of loads (24 values), over a thread's batches (up to 171 of the largest vocabulary) and within a warp, f64 from
 // the warps on: no more than 200 additions in a row. (All values of a thread in one row, 4096 of the largest vocabulary: ln s off by 6e-5.)
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(Logpr
         v[0] = load(p);
         take(v, p, 1);
       }
-    } else if (p < piece1) {  // at once, too (with alternatives that needs more than it saves: 344 us against 232 for 2048 rows of 128256)
+    } else if (p < piece1) {  // at once, too (with alternatives that needs more than it saves: 344 us against 232 for 2048 rows of 128256 and five of them)
       const int n = (int)((piece1 - p + kThreads - 1) / kThreads);
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
