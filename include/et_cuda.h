@@ -552,8 +552,8 @@ ETC_API etc_status etc_decoder_execute_sampled(etc_decoder* dec, etc_pool* pool,
 /* Scores a text: a step like etc_decoder_execute's (any advance up to the chunk length, same transaction) that returns, for every token
  * fed, the log probability of h_targets [active, advance] (the token that follows it) as etc_logprobs_into defines it, the entropy
  * (h_entropy may be NULL) and the `top` (0..32) most likely tokens [active, advance, top]. Norm and head run over all rows, some 256 at a
- * time, in a buffer that the first call makes. Results are written by steps that commit only. A vocabulary-parallel head is
- * ETC_UNSUPPORTED; a target outside the vocabulary is ETC_INVALID_ARGUMENT before any work. */
+ * time, in a buffer that the first call of several tokens per lane makes. Results are written by steps that commit only. A head of part of the
+ * vocabulary is ETC_UNSUPPORTED; a target outside the vocabulary is ETC_INVALID_ARGUMENT before any work. */
 ETC_API etc_status etc_decoder_score(etc_decoder* dec, etc_pool* pool, etc_seq* const* seqs, int active, const uint32_t* h_tokens,
                                      int advance, const uint32_t* h_targets, float* h_logprobs, float* h_entropy, int top,
                                      uint32_t* h_top_tokens, float* h_top_logprobs, const volatile int* cancelled);
